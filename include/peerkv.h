@@ -404,6 +404,110 @@ int pkv_rope_append(int device, const void* qkv, const int64_t* positions, const
 int pkv_swiglu(int device, const void* gate_up, void* out, int32_t rows, int32_t ffn,
                int32_t dtype, void* stream);
 
+/* ---- prompts, shared prefixes and their cache ------------------------------- */
+
+/* Attention of many query rows per sequence, packed sequences of different lengths, on one
+ * GPU: whole prompts, chunks of them behind cached tokens, single tokens in between, or (with
+ * causal = 0) groups of decoding sequences against the prefix they share.
+ *   q              [total_q, n_q_heads, 128], PKV_F16 or PKV_BF16; element strides between
+ *                  tokens and heads (multiples of 8, unit last stride), 16-byte aligned
+ *   cu_seqlens_q   [n_seqs + 1] int32: rows cu[i] .. cu[i+1] - 1 belong to sequence i, which may
+ *                  have none.  Rows behind the last sequence are not touched
+ *   paged K/V:  kv as in pkv_decode_args, 16-bit of q's type, page_size a multiple of 16;
+ *               block_table [n_seqs, block_table_stride] with block_table_cols usable
+ *               entries per row; seq_lens [n_seqs] tokens in the cache, the new ones included
+ *               (append first, then attend)
+ *   packed K/V: block_table and seq_lens NULL, cu_seqlens_k [n_seqs + 1]; kv.k / kv.v
+ *               [total keys, n_kv_heads, 128] described as one page of total-keys tokens
+ *   causal != 0: row r of n new rows sees keys j <= seq_len - n + r; a row that sees no key
+ *               gives O = 0 and lse = -inf
+ *   o_more, lse_more: NULL, or one more partial of the same rows ([total_q, n_q_heads, 128]
+ *               fp32 normalised, [total_q, n_q_heads] natural log) to fold into the result
+ *   scale          finite and > 0
+ * What the pool holds behind a sequence's last token is never used, not even when it is
+ * NaN; the tokens of a sequence must be finite in V, since a matrix instruction multiplies a
+ * hidden key of the same 128-key tile by a weight of 0.  n_q_heads / n_kv_heads <= 128.  A
+ * page id outside the pool is read as page 0 and sets PKV_ST_BAD_PAGE. */
+typedef struct pkv_prompt_args {
+  const void* q;
+  int64_t q_token_stride;
+  int64_t q_head_stride;
+  int32_t dtype;
+  int32_t n_q_heads;
+  int32_t total_q;
+  int32_t n_seqs;
+  const int32_t* cu_seqlens_q;
+  pkv_kv_view kv;
+  const int32_t* block_table;
+  int64_t block_table_stride;
+  int32_t block_table_cols;
+  int32_t causal;
+  const int32_t* seq_lens;
+  const int32_t* cu_seqlens_k;
+  const float* o_more;
+  const float* lse_more;
+  float scale;
+  int32_t reserved0;
+} pkv_prompt_args;
+
+/* Bytes of workspace one call needs on `device` (about 40 MB on a B200; 256-byte aligned device
+ * memory).  It holds nothing between calls: calls that may run at the same time need one each. */
+int pkv_prompt_workspace(int device, int64_t* bytes_out);
+
+/* out [total_q, n_q_heads, 128] in out_dtype (PKV_F16 / PKV_BF16 / PKV_F32); lse [total_q,
+ * n_q_heads] natural log, may be NULL; status_word a device word that bits are OR-ed into, may be
+ * NULL.  Allocates nothing, keeps nothing; the result does not depend on what else runs.
+ * The reference leaves prompts to its host engine; its shared-prefix batches are not fused
+ * (umallm/peerkv/vllm_backend.py:73-79 declines cascade batches). */
+int pkv_prompt_attention(int device, const pkv_prompt_args* a, void* out, int32_t out_dtype,
+                         float* lse, void* workspace, int64_t workspace_bytes,
+                         uint32_t* status_word, void* stream);
+
+/* New tokens on their way into the cache, one launch: per-head RMS norm of q and k, rotary
+ * positions, store of k and v by slot (pkv_rope_append for any number of tokens, norms,
+ * layouts, pool types and GPUs).
+ *   qkv        [n_tokens] rows, qkv_stride elements apart (multiple of 8): n_q_heads q heads,
+ *              n_kv_heads k heads, n_kv_heads v heads of 128 values, PKV_F16 or PKV_BF16
+ *   positions  [n_tokens] int64; inv_freq [rot_dim / 2] fp32 frequencies, scaled by the
+ *              caller for long contexts as it likes; gain multiplies cos and sin (1 = none);
+ *              rot_dim a multiple of 16, at most 128, 0 = no rotation: the first rot_dim values of a
+ *              head turn, the rest pass.  interleaved = 0: value i turns with i + rot_dim/2;
+ *              1: value 2i with 2i + 1.  The angle is reduced in 64 bits
+ *   q_weight, k_weight [128] of the same type, or NULL for no norm; y = x / sqrt(mean x^2 + eps) * w
+ *   q_out      [n_tokens, n_q_heads, 128], q_out_stride elements between tokens (multiple of
+ *              8); may be the q part of qkv itself
+ *   slot_mapping [n_tokens] int64 (page id * page_size + offset; negative = not stored), or
+ *              NULL for no append.  Slots of one call must differ
+ *   n_dev pools, pools[d] holding page ids bases[d] .. bases[d] + n_pages - 1 (the rule of
+ *              pkv_kv_append), all of one type: the 16-bit type of qkv, or PKV_INT8 /
+ *              PKV_FP8_E4M3 with k_scale / v_scale, which get what pkv_quantize_kv makes
+ *              of the 16-bit row.  Pools may lie in other GPUs' memory (P2P mapped)
+ * A slot outside every pool is skipped and sets PKV_ST_BAD_PAGE. */
+typedef struct pkv_append_args {
+  const void* qkv;
+  int64_t qkv_stride;
+  const int64_t* positions;
+  const float* inv_freq;
+  const void* q_weight;
+  const void* k_weight;
+  void* q_out;
+  int64_t q_out_stride;
+  const int64_t* slot_mapping;
+  const pkv_kv_view* pools;   /* host array of n_dev */
+  const int64_t* bases;       /* host array of n_dev */
+  int32_t n_dev;
+  int32_t n_tokens;
+  int32_t n_q_heads;
+  int32_t n_kv_heads;
+  int32_t head_dim;
+  int32_t dtype;
+  int32_t rot_dim;
+  int32_t interleaved;
+  float eps;
+  float gain;
+} pkv_append_args;
+int pkv_norm_rope_append(int device, const pkv_append_args* a, uint32_t* status_word, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -25,6 +25,7 @@ EXPORTS = [
     "pkv_add_rmsnorm", "pkv_rope_append", "pkv_swiglu", "pkv_kv_append",
     "pkv_enable_peer_access", "pkv_shard_stats", "pkv_prefill_partial", "pkv_stage_peer_blocks",
     "pkv_exchange_hop_probe", "pkv_exchange_hop_probe_reset",
+    "pkv_prompt_workspace", "pkv_prompt_attention", "pkv_norm_rope_append",
 ]
 
 
@@ -41,6 +42,25 @@ class DecodeArgs(C.Structure):
                 ("n_q_heads", C.c_int32), ("reserved0", C.c_int32), ("kv", KvView),
                 ("block_table", C.c_void_p), ("block_table_stride", C.c_int64),
                 ("seq_lens", C.c_void_p), ("scale", C.c_float), ("reserved1", C.c_int32)]
+
+
+class PromptArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64),
+                ("dtype", C.c_int32), ("n_q_heads", C.c_int32), ("total_q", C.c_int32), ("n_seqs", C.c_int32),
+                ("cu_seqlens_q", C.c_void_p), ("kv", KvView), ("block_table", C.c_void_p),
+                ("block_table_stride", C.c_int64), ("block_table_cols", C.c_int32), ("causal", C.c_int32),
+                ("seq_lens", C.c_void_p), ("cu_seqlens_k", C.c_void_p), ("o_more", C.c_void_p),
+                ("lse_more", C.c_void_p), ("scale", C.c_float), ("reserved0", C.c_int32)]
+
+
+class AppendArgs(C.Structure):
+    _fields_ = [("qkv", C.c_void_p), ("qkv_stride", C.c_int64), ("positions", C.c_void_p),
+                ("inv_freq", C.c_void_p), ("q_weight", C.c_void_p), ("k_weight", C.c_void_p),
+                ("q_out", C.c_void_p), ("q_out_stride", C.c_int64), ("slot_mapping", C.c_void_p),
+                ("pools", C.POINTER(KvView)), ("bases", C.POINTER(C.c_int64)), ("n_dev", C.c_int32),
+                ("n_tokens", C.c_int32), ("n_q_heads", C.c_int32), ("n_kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("dtype", C.c_int32), ("rot_dim", C.c_int32),
+                ("interleaved", C.c_int32), ("eps", C.c_float), ("gain", C.c_float)]
 
 
 class PeerKVError(RuntimeError):
@@ -103,6 +123,9 @@ def lib():
         "pkv_shard_stats": [vp, vp, P(u64), P(u64)],
         "pkv_stage_peer_blocks": [C.c_int, vp, i64, vp, i32, i32, i32, P(i64), P(i64), P(vp), P(vp), P(i64), vp, vp,
                                   i64, i64, i64, i64, i32, vp, vp, vp, vp],
+        "pkv_prompt_workspace": [C.c_int, P(i64)],
+        "pkv_prompt_attention": [C.c_int, P(PromptArgs), vp, i32, vp, vp, i64, vp, vp],
+        "pkv_norm_rope_append": [C.c_int, P(AppendArgs), vp, vp],
         "pkv_exchange_hop_probe": [vp, i32, i32, i32, i32, vp, vp],
         "pkv_exchange_hop_probe_reset": [vp, vp],
         "pkv_prefill_partial": [C.c_int, vp, i64, i64, i64, vp, vp, i64, i64, i64, i32, i32, i32, i32, i32, i32, i32,

@@ -10,12 +10,15 @@
 #include <cstring>
 #include <mutex>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/peerkv.h"
 #include "merge_kernel.cuh"
 #include "layer_kernels.cuh"
 #include "prefill_kernel.cuh"
+#include "prompt_kernel.cuh"
+#include "append_kernel.cuh"
 
 namespace {
 
@@ -1267,4 +1270,257 @@ extern "C" int pkv_static_status(int device, void* stream, uint32_t* status_out)
   int rc = static_setup(device);
   if (rc) return rc;
   return read_status(device, g_static_shard[device].status, static_cast<cudaStream_t>(stream), status_out);
+}
+
+// ------------------------------------------------------------------------- //
+// prompt attention, and the norm + rotation + append in front of it
+// ------------------------------------------------------------------------- //
+namespace {
+
+constexpr int kMaxDevices = 64;
+std::mutex g_prompt_mutex;
+int g_prompt_sms[kMaxDevices];         // SMs of a device once its kernels are set up
+
+// First call on a device: check it and raise the kernels' shared-memory limit.
+int prompt_setup(int device, int* sms_out) {
+  if (device < 0 || device >= kMaxDevices) return fail(PKV_E_INVALID, "device %d", device);
+  std::lock_guard<std::mutex> lock(g_prompt_mutex);
+  if (!g_prompt_sms[device]) {
+    DeviceGuard guard(device);
+    if (!guard.ok) return fail(PKV_E_CUDA, "cannot select device %d", device);
+    int sms = 0, major = 0;
+    PKV_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+    PKV_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
+    if (major != 10)
+      return fail(PKV_E_UNSUPPORTED, "device %d has compute capability %d.x; this library is sm_100a only", device, major);
+    int rc = set_smem(pkv::prompt_attn_kernel<true>, pkv::kPaSmem);
+    if (!rc) rc = set_smem(pkv::prompt_attn_kernel<false>, pkv::kPaSmem);
+    if (rc) return rc;
+    g_prompt_sms[device] = sms < pkv::kPaMaxCtas ? sms : pkv::kPaMaxCtas;
+  }
+  *sms_out = g_prompt_sms[device];
+  return PKV_OK;
+}
+
+struct PromptWorkspace { size_t o, ml, rec, bytes; };
+PromptWorkspace prompt_workspace(int n_cta) {
+  PromptWorkspace w;
+  w.o = 0;
+  w.ml = w.o + (size_t)2 * n_cta * 32 * 256 * sizeof(float4);
+  w.rec = w.ml + (size_t)2 * n_cta * 256 * sizeof(float2);
+  w.bytes = align_up(w.rec + (size_t)(n_cta + 1) * sizeof(pkv::PromptRec), 256);
+  return w;
+}
+
+int encode_map(CUtensorMap* out, int dtype, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+               const cuuint32_t* box, const char* what) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) return fail(PKV_E_CUDA, "cuTensorMapEncodeTiled entry point not available");
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = enc(out, dtype == PKV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+                   const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(PKV_E_CUDA, "cuTensorMapEncodeTiled failed (%d) for %s", (int)r, what);
+  return PKV_OK;
+}
+
+// A stride is only used between two elements of its dimension: with one element it may be anything.
+int64_t live_stride(int64_t stride, int64_t extent) { return extent > 1 ? stride : pkv::kHeadDim; }
+
+int check_stride(int64_t stride, int64_t extent, const char* what) {
+  if (extent > 1 && (stride <= 0 || stride % 8))
+    return fail(PKV_E_INVALID, "%s stride %lld: a positive multiple of 8 elements", what, (long long)stride);
+  return PKV_OK;
+}
+
+}  // namespace
+
+extern "C" int pkv_prompt_workspace(int device, int64_t* bytes_out) {
+  if (!bytes_out) return fail(PKV_E_INVALID, "null bytes_out");
+  int sms = 0;
+  int rc = prompt_setup(device, &sms);
+  if (rc) return rc;
+  *bytes_out = (int64_t)prompt_workspace(sms).bytes;
+  return PKV_OK;
+}
+
+extern "C" int pkv_prompt_attention(int device, const pkv_prompt_args* a, void* out, int32_t out_dtype, float* lse,
+                                    void* workspace, int64_t workspace_bytes, uint32_t* status_word, void* stream) {
+  if (!a) return fail(PKV_E_INVALID, "null args");
+  const pkv_kv_view& kv = a->kv;
+  if (kv.head_dim != pkv::kHeadDim) return fail(PKV_E_UNSUPPORTED, "head_dim %d: the kernels require 128", kv.head_dim);
+  if (!is_16bit(a->dtype)) return fail(PKV_E_INVALID, "dtype must be PKV_F16 or PKV_BF16");
+  if (kv.dtype != a->dtype) return fail(PKV_E_UNSUPPORTED, "K/V (%d) and q (%d) must share a 16-bit dtype", kv.dtype, a->dtype);
+  if (out_dtype != PKV_F16 && out_dtype != PKV_BF16 && out_dtype != PKV_F32) return fail(PKV_E_INVALID, "out_dtype %d", out_dtype);
+  if (a->n_q_heads <= 0 || kv.n_kv_heads <= 0 || a->n_q_heads % kv.n_kv_heads)
+    return fail(PKV_E_INVALID, "n_q_heads %d is not a multiple of n_kv_heads %d", a->n_q_heads, kv.n_kv_heads);
+  const int group = a->n_q_heads / kv.n_kv_heads;
+  if (group > pkv::kPaRows) return fail(PKV_E_UNSUPPORTED, "GQA group %d: at most 128 query heads per kv head", group);
+  if (a->total_q < 0 || a->n_seqs < 0) return fail(PKV_E_INVALID, "total_q %d n_seqs %d", a->total_q, a->n_seqs);
+  if (!(a->scale > 0.f) || a->scale > 1e30f) return fail(PKV_E_INVALID, "scale %g: finite and > 0", (double)a->scale);
+  if (a->total_q == 0 || a->n_seqs == 0) return PKV_OK;
+  if (!a->q || !a->cu_seqlens_q || !out || !workspace) return fail(PKV_E_INVALID, "null pointer");
+  if (!a->o_more != !a->lse_more) return fail(PKV_E_INVALID, "o_more and lse_more come together");
+  const bool paged = a->seq_lens != nullptr;
+  if (paged != (a->block_table != nullptr) || paged == (a->cu_seqlens_k != nullptr))
+    return fail(PKV_E_INVALID, "either block_table and seq_lens (paged) or cu_seqlens_k (packed)");
+  if (kv.n_pages < 0 || kv.page_size < 0 || kv.n_pages > 0x7fffffff) return fail(PKV_E_INVALID, "n_pages %lld page_size %d", (long long)kv.n_pages, kv.page_size);
+  if (paged) {
+    if (kv.page_size <= 0 || kv.page_size % 16) return fail(PKV_E_UNSUPPORTED, "page_size %d: a multiple of 16", kv.page_size);
+    if (a->block_table_cols < 0 || a->block_table_stride < 0) return fail(PKV_E_INVALID, "block_table_cols %d", a->block_table_cols);
+  } else if (kv.n_pages > 1) {
+    return fail(PKV_E_INVALID, "packed K/V is one page of all keys");
+  }
+  const bool any_keys = kv.n_pages > 0 && kv.page_size > 0;
+  int rc = PKV_OK;
+  if (any_keys) {
+    if (!kv.k || !kv.v) return fail(PKV_E_INVALID, "null k or v");
+    rc = check_stride(kv.token_stride, kv.page_size, "K/V token");
+    if (!rc) rc = check_stride(kv.head_stride, kv.n_kv_heads, "K/V head");
+    if (!rc) rc = check_stride(kv.page_stride, kv.n_pages, "K/V page");
+  }
+  if (!rc) rc = check_stride(a->q_token_stride, a->total_q, "q token");
+  if (!rc) rc = check_stride(a->q_head_stride, a->n_q_heads, "q head");
+  if (rc) return rc;
+  if ((reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(kv.k) | reinterpret_cast<uintptr_t>(kv.v) |
+       reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(a->o_more)) & 15)
+    return fail(PKV_E_INVALID, "q, k, v, out and o_more must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(workspace) & 255) return fail(PKV_E_INVALID, "workspace must be 256-byte aligned");
+  DeviceGuard guard(device);
+  if (!guard.ok) return fail(PKV_E_CUDA, "cannot select device %d", device);
+  int sms = 0;
+  rc = prompt_setup(device, &sms);
+  if (rc) return rc;
+  const PromptWorkspace ws = prompt_workspace(sms);
+  if (workspace_bytes < (int64_t)ws.bytes)
+    return fail(PKV_E_INVALID, "workspace of %lld bytes, %zu needed", (long long)workspace_bytes, ws.bytes);
+
+  pkv::PromptParams p;
+  memset(&p, 0, sizeof p);
+  p.cu_q = a->cu_seqlens_q; p.seq_lens = a->seq_lens; p.cu_k = a->cu_seqlens_k;
+  p.block_table = a->block_table; p.bt_stride = a->block_table_stride;
+  p.n_pages = kv.n_pages; p.page_size = kv.page_size;
+  p.table_cols = any_keys ? a->block_table_cols : 0;
+  p.total_k = any_keys && !paged ? kv.page_size : 0;
+  p.n_seq = a->n_seqs; p.total_q = a->total_q;
+  p.n_q_heads = a->n_q_heads; p.n_kv_heads = kv.n_kv_heads; p.group = group; p.tok_tile = pkv::kPaRows / group;
+  p.causal = a->causal ? 1 : 0;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.out = out; p.out_dtype = out_dtype; p.lse = lse; p.o_more = a->o_more; p.lse_more = a->lse_more;
+  uint8_t* wsb = static_cast<uint8_t*>(workspace);
+  p.part_o = reinterpret_cast<float4*>(wsb + ws.o);
+  p.part_ml = reinterpret_cast<float2*>(wsb + ws.ml);
+  p.rec = reinterpret_cast<pkv::PromptRec*>(wsb + ws.rec);
+  p.status = status_word;
+
+  CUtensorMap qm, km, vm;
+  memset(&km, 0, sizeof km);
+  memset(&vm, 0, sizeof vm);
+  {
+    const cuuint64_t dims[3] = {pkv::kHeadDim, (cuuint64_t)a->n_q_heads, (cuuint64_t)a->total_q};
+    const cuuint64_t strides[2] = {(cuuint64_t)live_stride(a->q_head_stride, a->n_q_heads) * 2,
+                                   (cuuint64_t)live_stride(a->q_token_stride, a->total_q) * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)p.tok_tile};
+    rc = encode_map(&qm, a->dtype, 3, a->q, dims, strides, box, "q");
+    if (rc) return rc;
+  }
+  // tokens per box: a power of two that divides a page, at most a tile; packed keys come whole
+  p.box_tok = pkv::kPaKeys;
+  if (paged) while (kv.page_size % p.box_tok) p.box_tok >>= 1;
+  if (any_keys) {
+    const int64_t ts = live_stride(kv.token_stride, kv.page_size), hs = live_stride(kv.head_stride, kv.n_kv_heads);
+    p.head_major = hs >= ts ? 1 : 0;
+    cuuint64_t dims[4] = {pkv::kHeadDim, (cuuint64_t)kv.n_kv_heads, (cuuint64_t)kv.page_size, (cuuint64_t)kv.n_pages};
+    cuuint64_t strides[3] = {(cuuint64_t)hs * 2, (cuuint64_t)ts * 2, (cuuint64_t)live_stride(kv.page_stride, kv.n_pages) * 2};
+    cuuint32_t box[4] = {64, 1, (cuuint32_t)p.box_tok, 1};
+    if (p.head_major) {
+      std::swap(dims[1], dims[2]);
+      std::swap(strides[0], strides[1]);
+      std::swap(box[1], box[2]);
+    }
+    rc = encode_map(&km, a->dtype, 4, kv.k, dims, strides, box, "k");
+    if (!rc) rc = encode_map(&vm, a->dtype, 4, kv.v, dims, strides, box, "v");
+    if (rc) return rc;
+  }
+
+  Range range("pkv:prompt_attention");
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof cfg);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // see griddepcontrol in the kernels
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3(sms);
+  cfg.blockDim = dim3(pkv::kPaThreads);
+  cfg.dynamicSmemBytes = pkv::kPaSmem;
+  if (a->dtype == PKV_BF16) PKV_CUDA(cudaLaunchKernelEx(&cfg, pkv::prompt_attn_kernel<true>, qm, km, vm, p));
+  else                      PKV_CUDA(cudaLaunchKernelEx(&cfg, pkv::prompt_attn_kernel<false>, qm, km, vm, p));
+  cfg.gridDim = dim3(sms - 1 > 0 ? sms - 1 : 1, 8);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  PKV_CUDA(cudaLaunchKernelEx(&cfg, pkv::prompt_join_kernel, p, sms));
+  PKV_CUDA(cudaGetLastError());
+  return PKV_OK;
+}
+
+extern "C" int pkv_norm_rope_append(int device, const pkv_append_args* a, uint32_t* status_word, void* stream) {
+  if (!a) return fail(PKV_E_INVALID, "null args");
+  if (a->head_dim != pkv::kHeadDim) return fail(PKV_E_UNSUPPORTED, "head_dim %d: 128 required", a->head_dim);
+  if (!is_16bit(a->dtype)) return fail(PKV_E_INVALID, "dtype must be PKV_F16 or PKV_BF16");
+  if (a->n_tokens < 0 || a->n_q_heads <= 0 || a->n_kv_heads <= 0 || a->n_q_heads > 65536 || a->n_kv_heads > 65536)
+    return fail(PKV_E_INVALID, "n_tokens %d heads %d/%d", a->n_tokens, a->n_q_heads, a->n_kv_heads);
+  if (a->rot_dim < 0 || a->rot_dim > pkv::kHeadDim || a->rot_dim % 16)
+    return fail(PKV_E_UNSUPPORTED, "rot_dim %d: a multiple of 16, at most 128", a->rot_dim);
+  if (!(a->eps >= 0.f)) return fail(PKV_E_INVALID, "eps %g", (double)a->eps);
+  if (a->n_tokens == 0) return PKV_OK;
+  if (!a->qkv || !a->q_out || (a->rot_dim > 0 && (!a->positions || !a->inv_freq))) return fail(PKV_E_INVALID, "null pointer");
+  if (a->qkv_stride % 8 || a->q_out_stride % 8) return fail(PKV_E_INVALID, "token strides must be multiples of 8 elements");
+  if ((reinterpret_cast<uintptr_t>(a->qkv) | reinterpret_cast<uintptr_t>(a->q_out) | reinterpret_cast<uintptr_t>(a->q_weight) |
+       reinterpret_cast<uintptr_t>(a->k_weight)) & 15)
+    return fail(PKV_E_INVALID, "qkv, q_out and the weights must be 16-byte aligned");
+  pkv::NormRopeParams p;
+  memset(&p, 0, sizeof p);
+  p.qkv = a->qkv; p.qkv_stride = a->qkv_stride; p.positions = a->positions; p.inv_freq = a->inv_freq;
+  p.q_weight = a->q_weight; p.k_weight = a->k_weight; p.q_out = a->q_out; p.q_stride = a->q_out_stride;
+  p.slot_mapping = a->slot_mapping;
+  p.n_tokens = a->n_tokens; p.n_q_heads = a->n_q_heads; p.n_kv_heads = a->n_kv_heads;
+  p.rot = a->rot_dim; p.interleaved = a->interleaved ? 1 : 0; p.eps = a->eps; p.gain = a->gain;
+  p.status = status_word;
+  if (a->slot_mapping) {
+    if (a->n_dev < 1 || a->n_dev > pkv::kMaxWorld || !a->pools || !a->bases) return fail(PKV_E_INVALID, "n_dev %d, pools and bases", a->n_dev);
+    p.n_dev = a->n_dev;
+    p.fmt = a->pools[0].dtype;
+    p.page_size = a->pools[0].page_size;
+    if (p.fmt != a->dtype && !is_quant(p.fmt))
+      return fail(PKV_E_INVALID, "pool dtype %d: that of qkv (%d), PKV_INT8 or PKV_FP8_E4M3", p.fmt, a->dtype);
+    if (p.page_size <= 0) return fail(PKV_E_INVALID, "page_size %d", p.page_size);
+    const uintptr_t align = is_quant(p.fmt) ? 7 : 15;
+    for (int d = 0; d < a->n_dev; ++d) {
+      const pkv_kv_view& v = a->pools[d];
+      if (v.dtype != p.fmt || v.page_size != p.page_size || v.n_kv_heads != a->n_kv_heads || v.head_dim != pkv::kHeadDim)
+        return fail(PKV_E_INVALID, "pool %d: dtype, page_size, n_kv_heads and head_dim must match", d);
+      if (v.n_pages < 0 || (v.n_pages > 0 && (!v.k || !v.v))) return fail(PKV_E_INVALID, "null pool %d", d);
+      if (is_quant(p.fmt) && v.n_pages > 0 && (!v.k_scale || !v.v_scale)) return fail(PKV_E_INVALID, "pool %d needs k_scale and v_scale", d);
+      if (d > 0 && a->bases[d] < a->bases[d - 1]) return fail(PKV_E_INVALID, "bases must ascend");
+      if (v.page_stride % 8 || v.token_stride % 8 || v.head_stride % 8 ||   // a lane stores eight values
+          ((reinterpret_cast<uintptr_t>(v.k) | reinterpret_cast<uintptr_t>(v.v)) & align))
+        return fail(PKV_E_INVALID, "pool %d: strides must be multiples of 8 elements and bases aligned to 8 of them", d);
+      p.bases[d] = a->bases[d]; p.n_pages[d] = v.n_pages;
+      p.k_pool[d] = static_cast<uint8_t*>(const_cast<void*>(v.k)); p.v_pool[d] = static_cast<uint8_t*>(const_cast<void*>(v.v));
+      p.k_scale[d] = static_cast<__half*>(const_cast<void*>(v.k_scale)); p.v_scale[d] = static_cast<__half*>(const_cast<void*>(v.v_scale));
+      p.page_stride[d] = v.page_stride; p.token_stride[d] = v.token_stride; p.head_stride[d] = v.head_stride;
+    }
+  }
+  DeviceGuard guard(device);
+  if (!guard.ok) return fail(PKV_E_CUDA, "cannot select device %d", device);
+  const int rows = p.n_q_heads + (p.slot_mapping ? 2 * p.n_kv_heads : 0);
+  const dim3 grid(p.n_tokens, (rows + pkv::kNraRows - 1) / pkv::kNraRows);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  Range range("pkv:norm_rope_append");
+  if (a->dtype == PKV_BF16) pkv::norm_rope_append_kernel<true><<<grid, pkv::kNraThreads, 0, st>>>(p);
+  else                      pkv::norm_rope_append_kernel<false><<<grid, pkv::kNraThreads, 0, st>>>(p);
+  PKV_CUDA(cudaGetLastError());
+  return PKV_OK;
 }

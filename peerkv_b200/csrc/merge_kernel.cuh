@@ -203,6 +203,25 @@ __global__ void __launch_bounds__(256) merge_partials_kernel(const MergeParams p
 //   a = max|x|; s32 = a/QMAX (1 if a == 0); stored scale s = fp16_rn(s32), bumped to
 //   the smallest fp16 subnormal if that rounded to 0; code = q(x / float(s)) with a
 //   true fp32 division; int8: rint + clamp to +-127; e4m3: clamp to +-448 then RNE.
+__device__ __forceinline__ __half kv_row_scale(float absmax, int fmt) {
+  const float qmax = fmt == 2 ? 127.f : 448.f;
+  float s32 = __fdiv_rn(absmax, qmax);
+  if (absmax == 0.f) s32 = 1.f;
+  __half s16 = __float2half_rn(s32);
+  if (__half2float(s16) == 0.f) s16 = __ushort_as_half((unsigned short)1);
+  return s16;
+}
+__device__ __forceinline__ uint32_t kv_code(float x, float scale, int fmt) {
+  const float y = __fdiv_rn(x, scale);
+  if (fmt == 2) {
+    const float r = fminf(fmaxf(rintf(y), -127.f), 127.f);
+    return static_cast<uint32_t>(static_cast<int>(r)) & 0xffu;
+  }
+  const float yc = fminf(fmaxf(y, -448.f), 448.f);
+  uint16_t pr;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(pr) : "f"(0.f), "f"(yc));
+  return pr & 0xffu;
+}
 template <bool BF16>
 __global__ void __launch_bounds__(256)
 quantize_kv_kernel(const void* __restrict__ src, int64_t rows, uint8_t* __restrict__ codes,
@@ -225,28 +244,11 @@ quantize_kv_kernel(const void* __restrict__ src, int64_t rows, uint8_t* __restri
   float a = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, off));
-  const float qmax = fmt == 2 ? 127.f : 448.f;
-  float s32 = __fdiv_rn(a, qmax);
-  if (a == 0.f) s32 = 1.f;
-  __half s16 = __float2half_rn(s32);
-  if (__half2float(s16) == 0.f) s16 = __ushort_as_half((unsigned short)1);
+  const __half s16 = kv_row_scale(a, fmt);
   const float sf = __half2float(s16);
   uint32_t packed = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float y = __fdiv_rn(x[i], sf);
-    uint32_t c;
-    if (fmt == 2) {
-      const float r = fminf(fmaxf(rintf(y), -127.f), 127.f);
-      c = static_cast<uint32_t>(static_cast<int>(r)) & 0xffu;
-    } else {
-      const float yc = fminf(fmaxf(y, -448.f), 448.f);
-      uint16_t pr;
-      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(pr) : "f"(0.f), "f"(yc));
-      c = pr & 0xffu;
-    }
-    packed |= c << (8 * i);
-  }
+  for (int i = 0; i < 4; ++i) packed |= kv_code(x[i], sf, fmt) << (8 * i);
   *(reinterpret_cast<uint32_t*>(codes + row * kHeadDim) + lane) = packed;
   if (lane == 0) scales[row] = s16;
 }

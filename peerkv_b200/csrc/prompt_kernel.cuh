@@ -1,0 +1,773 @@
+// Prompt attention: many query rows per sequence, packed sequences of different lengths, K/V
+// in the paged pool (or packed like the queries), on the fifth-generation tensor cores.  The
+// same kernel attends a group of decoding sequences to the prefix they share: the group is
+// one "sequence" whose query rows all see every key.
+//
+//   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i.k_j - m_i),  lse_i = m_i + log sum_j p_ij
+//   causal: query row i of n sees keys j <= L - n + i (the n rows are the last of L tokens).
+//
+// Tile.  128 rows = 128 / G tokens x the G query heads of one kv-head, so one K/V tile serves
+// the whole group and the causal diagonal of a tile is 128 / G tokens wide instead of 128.  A CTA
+// works on two row tiles at once (an "item" = 2 row tiles of one sequence and kv-head): while
+// one softmax warpgroup exponentiates, the tensor cores run the other's products.  An item
+// with a single row tile (few rows: a shared prefix, a chunk's end) gives the two warpgroups
+// alternate KV tiles instead and joins their accumulators at the end.
+//
+// Warps (384 threads, one CTA per SM): 0-3 and 4-7 the two softmax warpgroups, one thread per
+// row; 8 issues the TMA loads; 9 issues the tcgen05 instructions; 10-11 idle.
+// TMEM: S0 S1 O0 O1, 128 columns each; the 16-bit P overwrites the first half of its S.
+// Shared memory: Q 2 x 32 KB, a ring of five 32 KB slots that K and V tiles of 128 keys take
+// turns in (K0 V0 K1 V1 ..., the order in which the products need them).
+//
+// Sums.  Scores, maxima, sums and O are fp32.  P is rounded to the 16-bit type of V, as the
+// matrix instruction wants both operands alike; the row sum adds the unrounded values.  The
+// rounding costs an output as much as its own last rounding does (2^-9 relative per weight,
+// independent signs), half of the error budget of a 16-bit output.  The reference of the
+// exponentials moves only when a row's maximum has grown by more than 2^8: until then P
+// stays <= 256 and O need not be touched; l and lse use the same reference, so nothing is lost.
+//
+// Work split.  The KV tiles of all items form one list that is cut into equal pieces, one per
+// CTA, wherever the cut falls: ragged batches, causal triangles and a handful of rows over a
+// long cache are all balanced the same way.  An item that is cut leaves unnormalised (O, m, l)
+// pieces in a workspace which prompt_join_kernel adds up in a fixed order.
+#pragma once
+#include "decode_kernel.cuh"
+#include "tcgen05.cuh"
+
+namespace pkv {
+
+constexpr int kPaRows = 128;       // rows of a row tile (TMEM lanes)
+constexpr int kPaKeys = 128;       // keys of a KV tile
+constexpr int kPaThreads = 384;
+constexpr int kPaSlots = 5;
+constexpr int kPaTileBytes = kPaKeys * kHeadDim * 2;     // 32 KB
+constexpr int kPaHalfBytes = kPaTileBytes / 2;           // 128 rows x 64 values, 128-byte swizzle
+constexpr int kPaRingOff = 2 * kPaTileBytes;
+constexpr int kPaMiscOff = kPaRingOff + kPaSlots * kPaTileBytes;
+constexpr int kPaMiscBytes = 512 + 128 * 8;
+constexpr int kPaSmem = kPaMiscOff + kPaMiscBytes + 1024;  // 1 KB to align the base
+static_assert(kPaSmem <= 232448, "shared memory of a CTA");
+constexpr int kPaMaxCtas = 256;
+constexpr uint32_t kPaColO = 256;                        // TMEM columns: S0 0, S1 128, O0 256, O1 384
+constexpr int kPaItemCost = 192;   // what an item costs besides its keys, in keys
+constexpr int kPaMinPiece = 512;   // no CTA gets less than this many keys of work
+
+// Which CTA found which item cut (one per CTA, for the join).
+struct PromptRec {
+  int64_t a;             // start of the CTA's first item on the cost axis: the item's name
+  int mid;               // the CTA's piece starts inside that item
+  int kt0, kt1, n;       // the KV tiles of the item this CTA did, of n
+  int q0, n_tok, h;      // first packed row, tokens and kv-head of the item
+  int pad;
+};
+
+struct PromptParams {
+  const int32_t* cu_q;         // [n_seq + 1]
+  const int32_t* seq_lens;     // [n_seq] tokens in the cache; null: packed K/V, cu_k
+  const int32_t* cu_k;         // [n_seq + 1]
+  const int32_t* block_table;  // [n_seq][bt_stride]
+  int64_t bt_stride;
+  int64_t n_pages;
+  int table_cols;              // usable entries of a block-table row
+  int page_size, box_tok;      // tokens one TMA box brings (divides page_size and 128)
+  int head_major;
+  int n_seq, total_q, total_k;
+  int n_kv_heads, n_q_heads, group, tok_tile;   // tok_tile = 128 / group tokens per row tile
+  int causal;
+  float scale_log2;
+  void* out;                   // [total_q][n_q_heads][128]
+  int out_dtype;               // PKV_F16 / PKV_BF16 / PKV_F32
+  float* lse;                  // [total_q][n_q_heads] or null
+  const float* o_more;         // one more partial of the same rows to fold in, or null
+  const float* lse_more;
+  float4* part_o;              // workspace: [2 * CTAs][32][256]
+  float2* part_ml;             // [2 * CTAs][256]
+  PromptRec* rec;              // [CTAs + 1]; rec[CTAs].kt0 = CTAs in use
+  uint32_t* status;            // or null
+};
+
+// ---- the cost axis -------------------------------------------------------------------- //
+struct PromptSeq {
+  int q0, n, len, k0;          // packed first row, new tokens, cached tokens, first packed key
+  int tiles;                   // items per kv-head
+  int64_t step, add;           // item t costs add + step * (t + 1)
+};
+
+__device__ __forceinline__ PromptSeq prompt_seq(const PromptParams& p, int s) {
+  PromptSeq r;
+  const int lo = min(max(p.cu_q[s], 0), p.total_q), hi = min(max(p.cu_q[s + 1], lo), p.total_q);
+  r.q0 = lo;
+  r.n = hi - lo;
+  if (p.seq_lens) {
+    r.k0 = 0;
+    r.len = (int)min((int64_t)max(p.seq_lens[s], 0), (int64_t)p.table_cols * p.page_size);
+  } else {
+    r.k0 = min(max(p.cu_k[s], 0), p.total_k);
+    r.len = min(max(p.cu_k[s + 1], r.k0), p.total_k) - r.k0;
+  }
+  const int tt = 2 * p.tok_tile;
+  r.tiles = (r.n + tt - 1) / tt;
+  r.step = p.causal ? tt : 0;
+  r.add = (p.causal ? max(r.len - r.n, 0) : r.len) + kPaItemCost;
+  return r;
+}
+__device__ __forceinline__ int64_t prompt_items_cost(const PromptSeq& s, int64_t t) {   // of items 0 .. t-1
+  return t * s.add + s.step * (t * (t + 1) / 2);
+}
+
+struct PromptItem {
+  int s, h, t;                 // sequence, kv-head, item of the sequence
+  int64_t a, x0, x1;           // item's start on the cost axis; this CTA's piece of the axis
+  PromptSeq seq;
+  int q0, n_tok;               // first packed row, tokens of this item
+  int vis;                     // keys its last row sees
+  int n, kt0, kt1;             // KV tiles: of the item, and this CTA's share
+
+  // piece of a CTA -> tile index: monotone, 0 at the item's start, n at its end
+  __device__ __forceinline__ int cut(int64_t y, int64_t cost) const {
+    return y <= 0 ? 0 : y >= cost ? n : (int)(y * n / cost);
+  }
+  __device__ __forceinline__ void fill(const PromptParams& p) {
+    const int tt = 2 * p.tok_tile;
+    q0 = seq.q0 + t * tt;
+    n_tok = min(tt, seq.n - t * tt);
+    vis = p.causal ? max(0, min(seq.len, seq.len - seq.n + t * tt + n_tok)) : seq.len;
+    n = (vis + kPaKeys - 1) / kPaKeys;
+    const int64_t cost = seq.add + seq.step * (t + 1);
+    kt0 = cut(x0 - a, cost);
+    kt1 = cut(x1 - a, cost);
+  }
+  // first item of the piece: s and `base` (cost before sequence s) are known
+  __device__ __forceinline__ void start(const PromptParams& p, int64_t base) {
+    seq = prompt_seq(p, s);
+    const int64_t per = prompt_items_cost(seq, seq.tiles);
+    h = (int)((x0 - base) / per);
+    const int64_t y = x0 - base - h * per;
+    int lo = 0, hi = seq.tiles - 1;                      // largest t with cost(0 .. t-1) <= y
+    while (lo < hi) {
+      const int m = (lo + hi + 1) >> 1;
+      if (prompt_items_cost(seq, m) <= y) lo = m; else hi = m - 1;
+    }
+    t = lo;
+    a = base + h * per + prompt_items_cost(seq, t);
+    fill(p);
+  }
+  // the next item; false when the piece is done
+  __device__ __forceinline__ bool next(const PromptParams& p) {
+    a += seq.add + seq.step * (t + 1);
+    if (a >= x1) return false;
+    if (++t == seq.tiles) {
+      t = 0;
+      if (++h == p.n_kv_heads) {
+        h = 0;
+        do {
+          if (++s >= p.n_seq) return false;
+          seq = prompt_seq(p, s);
+        } while (seq.tiles == 0);
+      }
+    }
+    fill(p);
+    return true;
+  }
+  // this CTA has tiles of the item, or the item has none and starts here
+  __device__ __forceinline__ bool mine() const { return kt1 > kt0 || (n == 0 && x0 <= a); }
+  __device__ __forceinline__ bool whole() const { return kt0 == 0 && kt1 == n; }
+  __device__ __forceinline__ bool two(const PromptParams& p) const { return n_tok > p.tok_tile; }
+};
+
+// ---- bounded waits -------------------------------------------------------------------- //
+// A step of the pipeline takes microseconds; a wait that has not ended after two seconds sets
+// the abort flag, every later wait returns at once, and the CTA runs out.
+__device__ __forceinline__ bool pa_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {   // whole warp
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  unsigned long long t0 = 0;
+  for (uint32_t w = 0;; ++w) {       // every exit is taken by all lanes together
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, *abort_flag)) return false;
+    if ((w & 63u) == 63u) {
+      const unsigned long long now = global_ns();
+      if (t0 == 0) t0 = now;
+      if (__any_sync(0xffffffffu, now - t0 > 2000000000ull)) { *abort_flag = 1; return false; }
+    }
+  }
+}
+
+__device__ __forceinline__ void store_row16(void* row, int out_dtype, int chunk, const float (&v)[8]) {
+  // eight values of a row at column 8 * chunk
+  if (out_dtype == 4) {
+    float4* d = reinterpret_cast<float4*>(row) + chunk * 2;
+    d[0] = make_float4(v[0], v[1], v[2], v[3]);
+    d[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    uint4 w;
+    if (out_dtype == 1) { w.x = pack2<true>(v[0], v[1]); w.y = pack2<true>(v[2], v[3]); w.z = pack2<true>(v[4], v[5]); w.w = pack2<true>(v[6], v[7]); }
+    else { w.x = pack2<false>(v[0], v[1]); w.y = pack2<false>(v[2], v[3]); w.z = pack2<false>(v[4], v[5]); w.w = pack2<false>(v[6], v[7]); }
+    reinterpret_cast<uint4*>(row)[chunk] = w;
+  }
+}
+
+template <bool BF16>
+__global__ void __launch_bounds__(kPaThreads, 1)
+prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                   const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PromptParams p) {
+  extern __shared__ uint8_t pa_raw[];
+  uint8_t* sgen = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pa_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t smem = smem_u32(sgen);
+  uint8_t* misc = sgen + kPaMiscOff;
+  const uint32_t bars = smem + kPaMiscOff;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  auto full = [&](int i) { return bars + 8u * i; };
+  auto empty = [&](int i) { return bars + 8u * (kPaSlots + i); };
+  const uint32_t q_full = bars + 8u * 10, q_empty = bars + 8u * 11, done = bars + 8u * 12;
+  auto s_full = [&](int w) { return bars + 8u * (13 + w); };
+  auto p_full = [&](int w) { return bars + 8u * (15 + w); };
+  auto o_full = [&](int w) { return bars + 8u * (17 + w); };
+  const uint32_t x_ready = bars + 8u * 19, x_done = bars + 8u * 20;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 192);
+  uint32_t* tmem_word = reinterpret_cast<uint32_t*>(misc + 196);
+  volatile int64_t* first = reinterpret_cast<volatile int64_t*>(misc + 208);   // s, base, total
+  int64_t* wsum = reinterpret_cast<int64_t*>(misc + 256);                      // 12 warp sums
+  float2* xml = reinterpret_cast<float2*>(misc + 512);                         // [128] (m, l) of stream 1
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kPaSlots; ++i) { mbar_init(full(i), 1); mbar_init(empty(i), 1); }
+    mbar_init(q_full, 1); mbar_init(q_empty, 1); mbar_init(done, 1);
+    for (int w = 0; w < 2; ++w) { mbar_init(s_full(w), 1); mbar_init(p_full(w), 4); mbar_init(o_full(w), 1); }
+    mbar_init(x_ready, 4); mbar_init(x_done, 4);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 8) tmem_alloc(smem_u32(tmem_word), 512);
+  if (warp == 9 && lane == 0) { prefetch_tensormap(&qmap); prefetch_tensormap(&kmap); prefetch_tensormap(&vmap); }
+  // Launched with programmatic stream serialisation: nothing of global memory is read above.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // ---- this CTA's piece of the cost axis ----
+  const int per_thread = (p.n_seq + kPaThreads - 1) / kPaThreads;
+  const int sb = min((int)threadIdx.x * per_thread, p.n_seq), se = min(sb + per_thread, p.n_seq);
+  int64_t mine = 0;
+  for (int s = sb; s < se; ++s) {
+    const PromptSeq q = prompt_seq(p, s);
+    mine += p.n_kv_heads * prompt_items_cost(q, q.tiles);
+  }
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) wsum[warp] = incl;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  int64_t before = incl - mine, total = 0;
+  for (int w = 0; w < kPaThreads / 32; ++w) {
+    if (w < warp) before += wsum[w];
+    total += wsum[w];
+  }
+  const int n_cta = (int)min((int64_t)gridDim.x, (total + kPaMinPiece - 1) / kPaMinPiece);
+  const bool active = (int)blockIdx.x < n_cta;
+  PromptItem it;
+  it.x0 = active ? total * blockIdx.x / n_cta : 0;
+  it.x1 = active ? total * (blockIdx.x + 1) / n_cta : 0;
+  if (active && before <= it.x0 && it.x0 < before + mine) {
+    int64_t base = before;
+    for (int s = sb; s < se; ++s) {
+      const PromptSeq q = prompt_seq(p, s);
+      const int64_t c = p.n_kv_heads * prompt_items_cost(q, q.tiles);
+      if (it.x0 < base + c) { first[0] = s; first[1] = base; break; }
+      base += c;
+    }
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.rec[gridDim.x].kt0 = n_cta;
+  __syncthreads();
+  const uint32_t tmem = *tmem_word;
+
+  if (active) {
+    it.s = (int)first[0];
+    it.start(p, first[1]);
+    if (threadIdx.x == 0) {
+      PromptRec r;
+      r.a = it.a; r.mid = it.x0 > it.a ? 1 : 0; r.kt0 = it.kt0; r.kt1 = it.kt1; r.n = it.n;
+      r.q0 = it.q0; r.n_tok = it.n_tok; r.h = it.h; r.pad = 0;
+      p.rec[blockIdx.x] = r;
+    }
+  }
+
+  if (active && warp < 8) {
+    // ------------------------------ softmax warpgroups ------------------------------ //
+    const int w = warp >> 2, row = threadIdx.x & 127;
+    const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);      // lane 32 * (warp % 4)
+    const uint32_t ts = lane_base + w * 128, to = lane_base + kPaColO + w * 128;
+    const int tok_in = row / p.group, head_in = row - tok_in * p.group;
+    const float sl = p.scale_log2;
+    uint32_t n_s = 0, n_o = 0, n_x = 0;                                   // barrier phases used
+    bool ok = true;
+    do {
+      if (!it.mine()) continue;
+      const bool two = it.two(p);
+      const int tok = (two ? w * p.tok_tile : 0) + tok_in;               // token of this row in the item
+      const int n_tiles = it.kt1 - it.kt0;
+      const int steps = two ? n_tiles : (n_tiles + 1 - w) >> 1;          // one row tile: alternate KV tiles
+      // keys [0, lim) are visible to this row
+      const int lim = p.causal ? min(it.seq.len, it.seq.len - it.seq.n + (it.q0 - it.seq.q0) + tok + 1) : it.seq.len;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < steps; ++j) {
+        const int key0 = (it.kt0 + (two ? j : 2 * j + w)) * kPaKeys;
+        if (!(ok = pa_wait(s_full(w), n_s & 1, abort_flag))) break;
+        ++n_s;
+        tc_fence_after();
+        uint32_t sreg[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(sreg[c], ts + c * 32);
+        tmem_wait_ld();
+        if (__any_sync(0xffffffffu, key0 + kPaKeys > lim)) {
+          const int left = lim - key0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c * 32 + i >= left) sreg[c][i] = 0xff800000u;           // -inf
+        }
+        float mx[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          mx[c] = __uint_as_float(sreg[c][0]);
+#pragma unroll
+          for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(sreg[c][i]));
+        }
+        const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if (j == 0) {
+          m = tile_max;
+        } else if (__any_sync(0xffffffffu, (tile_max - m) * sl > 8.f)) {
+          // The product that wrote O last is complete: the scores just waited for were issued
+          // behind it, and the next one waits for this warpgroup.
+          const float mn = fmaxf(m, tile_max);
+          const float alpha = m == -INFINITY ? 0.f : fast_exp2((m - mn) * sl);
+          l *= alpha;
+          m = mn;
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld32(o, to + c * 32);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st32(to + c * 32, o);
+          }
+        }
+        // a row that has seen no key yet has m = -inf: 0 as the reference keeps exp2(-inf) = 0
+        const float ref = m == -INFINITY ? 0.f : -m * sl;
+        float sum0 = 0.f, sum1 = 0.f, sum2 = 0.f, sum3 = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float e0 = fast_exp2(fmaf(__uint_as_float(sreg[c][i]), sl, ref));
+            const float e1 = fast_exp2(fmaf(__uint_as_float(sreg[c][i + 1]), sl, ref));
+            const float e2 = fast_exp2(fmaf(__uint_as_float(sreg[c][i + 2]), sl, ref));
+            const float e3 = fast_exp2(fmaf(__uint_as_float(sreg[c][i + 3]), sl, ref));
+            sum0 += e0; sum1 += e1; sum2 += e2; sum3 += e3;
+            pk[i / 2] = pack2<BF16>(e0, e1);
+            pk[i / 2 + 1] = pack2<BF16>(e2, e3);
+          }
+          tmem_st16(ts + c * 16, pk);
+        }
+        l += (sum0 + sum1) + (sum2 + sum3);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full(w));
+      }
+      if (!ok) break;
+
+      // ---- epilogue ----
+      float a0 = 1.f, a1 = 0.f;                 // weights of O_w and (one row tile) of the other stream's O
+      bool join = false;
+      if (steps > 0) {
+        if (!(ok = pa_wait(o_full(w), n_o & 1, abort_flag))) break;
+        ++n_o;
+        tc_fence_after();
+      }
+      if (!two && n_tiles > 1) {
+        if (w == 1) {
+          xml[row] = make_float2(m, l);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(x_ready);
+          if (!(ok = pa_wait(x_done, n_x & 1, abort_flag))) break;   // O1 and xml are free again
+          ++n_x;
+        } else {
+          if (!(ok = pa_wait(x_ready, n_x & 1, abort_flag))) break;
+          ++n_x;
+          tc_fence_after();
+          const float2 other = xml[row];
+          const float mn = fmaxf(m, other.x);
+          a0 = m == -INFINITY ? 0.f : fast_exp2((m - mn) * sl);
+          a1 = other.x == -INFINITY ? 0.f : fast_exp2((other.x - mn) * sl);
+          l = l * a0 + other.y * a1;
+          m = mn;
+          join = true;
+        }
+      }
+      if (two || w == 0) {
+        const bool valid = tok < it.n_tok && row < p.tok_tile * p.group;
+        const bool whole = it.whole();
+        const int64_t orow = (int64_t)(it.q0 + tok) * p.n_q_heads + it.h * p.group + head_in;
+        const float m2 = m == -INFINITY ? -INFINITY : m * sl;           // base-2 units
+        float wa = l > 0.f ? 1.f / l : 0.f, wb = 0.f;
+        if (l != l) wa = l;                                            // NaN scores stay NaN
+        if (whole && valid) {
+          float lse2 = l > 0.f ? m2 + log2f(l) : (l != l ? l : -INFINITY);
+          if (p.o_more) {
+            const float b2 = p.lse_more[orow] * 1.4426950408889634f;
+            const float top = fmaxf(lse2, b2);
+            const float ea = lse2 == -INFINITY ? 0.f : exp2f(lse2 - top), eb = b2 == -INFINITY ? 0.f : exp2f(b2 - top);
+            const float s = ea + eb, inv = s > 0.f ? 1.f / s : 0.f;
+            wa *= ea * inv;
+            wb = eb * inv;
+            lse2 = s > 0.f ? top + log2f(s) : -INFINITY;
+          }
+          if (p.lse) p.lse[orow] = lse2 * 0.6931471805599453f;
+        }
+        const int slot = 2 * blockIdx.x + (it.x0 > it.a ? 0 : 1);
+        const int prow = (two ? w * kPaRows : 0) + row;
+        if (!whole) p.part_ml[(size_t)slot * 256 + prow] = make_float2(m2, l);
+        float4* po = p.part_o + (size_t)slot * 32 * 256 + prow;
+        uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + orow * kHeadDim * (p.out_dtype == 4 ? 4 : 2);
+        const float* more = p.o_more ? p.o_more + orow * kHeadDim : nullptr;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          if (steps > 0) {
+            tmem_ld32(o, to + c * 32);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0u;
+          }
+          if (join) {
+            uint32_t o1[32];
+            tmem_ld32(o1, to + 128 + c * 32);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              o[i] = __float_as_uint(__uint_as_float(o[i]) * a0 + __uint_as_float(o1[i]) * a1);
+          }
+          if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              po[(c * 8 + i) * 256] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                                  __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+          } else if (valid) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float v[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                v[e] = __uint_as_float(o[8 * i + e]) * wa;
+                if (more && wb != 0.f) v[e] = fmaf(more[c * 32 + i * 8 + e], wb, v[e]);
+              }
+              store_row16(dst, p.out_dtype, c * 4 + i, v);
+            }
+          }
+        }
+        tc_fence_before();
+        if (join) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(x_done);
+        }
+      }
+    } while (it.next(p));
+  } else if (active && warp == 8) {
+    // ------------------------------------ loads ------------------------------------ //
+    const int boxes = kPaKeys / p.box_tok;              // of one half tile
+    const uint32_t box_bytes = (uint32_t)p.box_tok * 128u;
+    const bool paged = p.seq_lens != nullptr;
+    uint32_t n_tile = 0, n_q = 0;
+    bool ok = true;
+    do {
+      if (!it.mine() || it.kt1 == it.kt0) continue;
+      const bool two = it.two(p);
+      const int n_tiles = it.kt1 - it.kt0;
+      // Q: the group's heads of up to 2 * tok_tile tokens, in two halves of 64 values
+      if (!(ok = pa_wait(q_empty, (n_q & 1) ^ 1, abort_flag))) break;
+      ++n_q;
+      if (lane == 0) {
+        const uint32_t half = (uint32_t)p.tok_tile * p.group * 128u;
+        mbar_arrive_expect_tx(q_full, half * (two ? 4u : 2u));
+        for (int w = 0; w < (two ? 2 : 1); ++w)
+          for (int d = 0; d < 2; ++d)
+            tma_load_3d(smem + w * kPaTileBytes + d * kPaHalfBytes, &qmap, q_full, d * 64, it.h * p.group,
+                        it.q0 + w * p.tok_tile);
+      }
+      __syncwarp();
+      const int32_t* row = paged ? p.block_table + (int64_t)it.s * p.bt_stride : nullptr;
+      // one tile of K (kv = 0) or V (kv = 1): lane = 2 * box + half
+      auto load = [&](int kt, int kv) {
+        const int slot = n_tile % kPaSlots;
+        if (!pa_wait(empty(slot), ((n_tile / kPaSlots) & 1) ^ 1, abort_flag)) return false;
+        ++n_tile;
+        const int key0 = kt * kPaKeys;
+        const int n_box = min(boxes, (it.vis - key0 + p.box_tok - 1) / p.box_tok);   // >= 1
+        const uint32_t dst0 = smem + kPaRingOff + slot * kPaTileBytes;
+        const CUtensorMap* map = kv ? &vmap : &kmap;
+        if (lane == 0) mbar_arrive_expect_tx(full(slot), n_box * 2 * box_bytes);
+        __syncwarp();
+        if (lane < 2 * n_box) {
+          const int b = lane >> 1, d = lane & 1;
+          const uint32_t dst = dst0 + d * kPaHalfBytes + b * box_bytes;
+          if (paged) {
+            const int key = key0 + b * p.box_tok, pg = key / p.page_size, tok = key - pg * p.page_size;
+            int page = row[pg];
+            if (page < 0 || page >= p.n_pages) {
+              if (p.status) atomicOr(p.status, kStBadPage);
+              page = 0;
+            }
+            if (p.head_major) tma_load_4d_keep(dst, map, full(slot), d * 64, tok, it.h, page);
+            else              tma_load_4d_keep(dst, map, full(slot), d * 64, it.h, tok, page);
+          } else {
+            tma_load_4d_keep(dst, map, full(slot), d * 64, it.h, it.seq.k0 + key0, 0);
+          }
+        }
+        __syncwarp();
+        return true;
+      };
+      if (two) {
+        for (int kt = it.kt0; kt < it.kt1 && ok; ++kt) ok = load(kt, 0) && load(kt, 1);
+      } else {
+        ok = load(it.kt0, 0) && (n_tiles < 2 || load(it.kt0 + 1, 0));
+        for (int i = 0; i < n_tiles && ok; ++i)
+          ok = load(it.kt0 + i, 1) && (i + 2 >= n_tiles || load(it.kt0 + i + 2, 0));
+      }
+    } while (ok && it.next(p));
+    if (!ok) {       // give the copies in flight a bounded chance to land before the CTA goes away
+      for (uint32_t back = 1; back <= (uint32_t)kPaSlots && back <= n_tile; ++back) {
+        const uint32_t i = n_tile - back;
+        mbar_wait_bounded(full(i % kPaSlots), (i / kPaSlots) & 1, kPollLimit);
+      }
+      if (n_q) mbar_wait_bounded(q_full, (n_q - 1) & 1, kPollLimit);
+    }
+  } else if (active && warp == 9) {
+    // ------------------------------- matrix instructions ----------------------------- //
+    // The warp stays together; lane 0 issues.
+    constexpr uint32_t idesc_qk = umma_idesc(BF16, false, kPaRows, kPaKeys);
+    constexpr uint32_t idesc_pv = umma_idesc(BF16, true, kPaRows, kHeadDim);
+    uint32_t n_tile = 0, n_q = 0, n_p0 = 0, n_p1 = 0;
+    bool ok = true;
+    auto slot_of = [&](uint32_t i) { return smem + kPaRingOff + (i % kPaSlots) * kPaTileBytes; };
+    auto wait_tile = [&](uint32_t i) { return pa_wait(full(i % kPaSlots), (i / kPaSlots) & 1, abort_flag); };
+    auto qk = [&](int w, int qtile, uint32_t i) {         // S_w = Q K^T
+      if (lane == 0) {
+        const uint32_t qa = smem + qtile * kPaTileBytes, ka = slot_of(i);
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          const uint32_t off = (ks >> 2) * kPaHalfBytes + (ks & 3) * 32;
+          umma_ss(tmem + w * 128, umma_desc(qa + off, 16, 1024), umma_desc(ka + off, 16, 1024), idesc_qk, ks > 0);
+        }
+        umma_commit(s_full(w));
+      }
+      __syncwarp();
+    };
+    auto pv = [&](int w, uint32_t i, int ksteps, bool first_tile) {   // O_w (+)= P_w V
+      if (lane == 0) {
+        const uint32_t va = slot_of(i);
+        for (int ks = 0; ks < ksteps; ++ks)
+          umma_ts(tmem + kPaColO + w * 128, tmem + w * 128 + ks * 8, umma_desc(va + ks * 2048, kPaHalfBytes, 1024),
+                  idesc_pv, !first_tile || ks > 0);
+      }
+      __syncwarp();
+    };
+    // V rows of the last 16-key step that lie behind the sequence hold whatever the page holds:
+    // their weights are 0, but 0 * NaN is not, so they are cleared in shared memory.
+    auto clean = [&](uint32_t i, int kt, int ksteps) {
+      const int from = it.seq.len - kt * kPaKeys, to = ksteps * 16;
+      if (from >= to) return;
+      uint8_t* v = sgen + kPaRingOff + (i % kPaSlots) * kPaTileBytes;
+      for (int r = max(from, 0); r < to; ++r) {
+        *reinterpret_cast<uint32_t*>(v + r * 128 + lane * 4) = 0u;
+        *reinterpret_cast<uint32_t*>(v + kPaHalfBytes + r * 128 + lane * 4) = 0u;
+      }
+      fence_proxy_async();
+      __syncwarp();
+    };
+    auto steps_of = [&](int kt) { return min(8, (it.vis - kt * kPaKeys + 15) >> 4); };
+    auto wait_p = [&](int w) {
+      const bool r = w ? pa_wait(p_full(1), n_p1 & 1, abort_flag) : pa_wait(p_full(0), n_p0 & 1, abort_flag);
+      if (w) ++n_p1; else ++n_p0;
+      if (r) tc_fence_after();
+      return r;
+    };
+    auto commit = [&](uint32_t bar) { if (lane == 0) umma_commit(bar); };
+    do {
+      if (!it.mine() || it.kt1 == it.kt0) continue;
+      const bool two = it.two(p);
+      const int n_tiles = it.kt1 - it.kt0;
+      if (!(ok = pa_wait(q_full, n_q & 1, abort_flag))) break;
+      ++n_q;
+      if (two) {
+        // ring order K0 V0 K1 V1 ...: tile j's K is entry base + 2j, its V base + 2j + 1
+        const uint32_t base = n_tile;
+        n_tile += 2 * n_tiles;
+        if (!(ok = wait_tile(base))) break;
+        qk(0, 0, base);
+        qk(1, 1, base);
+        commit(empty(base % kPaSlots));
+        if (n_tiles == 1) commit(q_empty);
+        for (int j = 0; j < n_tiles; ++j) {
+          const int kt = it.kt0 + j, ks = steps_of(kt);
+          const uint32_t iv = base + 2 * j + 1, ik = iv + 1;
+          const bool more = j + 1 < n_tiles;
+          if (!(ok = wait_tile(iv))) break;
+          clean(iv, kt, ks);
+          if (!(ok = wait_p(0))) break;
+          pv(0, iv, ks, j == 0);
+          if (more) {
+            if (!(ok = wait_tile(ik))) break;
+            qk(0, 0, ik);
+          } else {
+            commit(o_full(0));
+          }
+          if (!(ok = wait_p(1))) break;
+          pv(1, iv, ks, j == 0);
+          commit(empty(iv % kPaSlots));
+          if (more) {
+            qk(1, 1, ik);
+            commit(empty(ik % kPaSlots));
+            if (j + 2 == n_tiles) commit(q_empty);
+          } else {
+            commit(o_full(1));
+          }
+        }
+      } else {
+        // one row tile: stream w takes tiles w, w + 2, ...; ring order K0 K1 V0 K2 V1 K3 V2 ...
+        const uint32_t base = n_tile;
+        n_tile += 2 * n_tiles;
+        auto k_at = [&](int i) { return base + (i < 2 ? (uint32_t)i : 2u * i - 1u); };
+        auto v_at = [&](int i) {      // V_i follows K_{i+1} where that exists
+          return base + (i + 1 < n_tiles ? 2u * i + 2u : 2u * i + 1u);
+        };
+        for (int i = 0; i < min(2, n_tiles); ++i) {
+          if (!(ok = wait_tile(k_at(i)))) break;
+          qk(i, 0, k_at(i));
+          commit(empty(k_at(i) % kPaSlots));
+        }
+        if (!ok) break;
+        if (n_tiles <= 2) commit(q_empty);
+        for (int i = 0; i < n_tiles; ++i) {
+          const int w = i & 1, kt = it.kt0 + i, ks = steps_of(kt);
+          const uint32_t iv = v_at(i);
+          if (!(ok = wait_tile(iv))) break;
+          clean(iv, kt, ks);
+          if (!(ok = wait_p(w))) break;
+          pv(w, iv, ks, i < 2);
+          commit(empty(iv % kPaSlots));
+          if (i + 2 >= n_tiles) {
+            commit(o_full(w));
+          } else {
+            const uint32_t ik = k_at(i + 2);
+            if (!(ok = wait_tile(ik))) break;
+            qk(w, 0, ik);
+            commit(empty(ik % kPaSlots));
+            if (i + 3 == n_tiles) commit(q_empty);
+          }
+        }
+      }
+    } while (ok && it.next(p));
+    // everything issued is complete, and its arrivals have landed, before the CTA goes away
+    commit(done);
+    mbar_wait_bounded(done, 0, kPollLimit);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag && p.status) atomicOr(p.status, kStPipeTimeout);
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Adds up the pieces of the items that were cut, in the order of their keys.  Block (c, y):
+// the item in which CTA c's piece starts, if c is the first CTA to start inside it; one thread
+// per row, 16 of the 128 values.  The pieces are a few MB that were written a moment ago: L2.
+__global__ void __launch_bounds__(256) prompt_join_kernel(const PromptParams p, int n_grid) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int c = blockIdx.x + 1, row = threadIdx.x;
+  const int n_cta = p.rec[n_grid].kt0;
+  if (c >= n_cta) return;
+  const PromptRec r = p.rec[c];
+  if (!r.mid || r.kt0 >= r.n) return;                       // not inside an item, or all of it was done before
+  if (c > 1) {
+    const PromptRec b = p.rec[c - 1];
+    if (b.mid && b.a == r.a) return;                        // an earlier CTA starts inside it too
+  }
+  if (r.kt0 == 0 && r.kt1 == r.n) return;                   // this CTA did all of it
+  int last = c;                                             // last CTA that starts inside the item
+  while (last + 1 < n_cta) {
+    const PromptRec b = p.rec[last + 1];
+    if (!b.mid || b.a != r.a) break;
+    if (b.kt0 == 0 && b.kt1 == b.n) return;
+    ++last;
+  }
+  const bool two = r.n_tok > p.tok_tile;
+  const int w = row >> 7, lr = row & 127;
+  if (w && !two) return;
+  const int tok_in = lr / p.group, head_in = lr - tok_in * p.group, tok = w * p.tok_tile + tok_in;
+  if (lr >= p.tok_tile * p.group || tok >= r.n_tok) return;
+  const int64_t orow = (int64_t)(r.q0 + tok) * p.n_q_heads + r.h * p.group + head_in;
+
+  // piece i: the CTA before c (its last item), then c .. last (their first items)
+  auto slot_of = [&](int i) { return i == 0 ? 2 * (c - 1) + 1 : 2 * (c + i - 1); };
+  auto has = [&](int i) {
+    if (i == 0) return r.kt0 > 0;
+    const PromptRec& b = p.rec[c + i - 1];
+    return b.kt1 > b.kt0;
+  };
+  const int n = last - c + 2;
+  float m = -INFINITY;
+  for (int i = 0; i < n; ++i)
+    if (has(i)) m = fmaxf(m, p.part_ml[(size_t)slot_of(i) * 256 + row].x);
+  float b2 = -INFINITY;
+  if (p.o_more) {
+    b2 = p.lse_more[orow] * 1.4426950408889634f;
+    m = fmaxf(m, b2);
+  }
+  float l = 0.f, acc[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+  for (int i = 0; i < n; ++i) {
+    if (!has(i)) continue;
+    const float2 ml = p.part_ml[(size_t)slot_of(i) * 256 + row];
+    const float f = ml.x == -INFINITY ? (ml.y == ml.y ? 0.f : ml.y) : exp2f(ml.x - m);
+    l += ml.y * f;
+    const float4* po = p.part_o + (size_t)slot_of(i) * 32 * 256 + row;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float4 v = po[(blockIdx.y * 4 + e) * 256];
+      acc[4 * e] += v.x * f; acc[4 * e + 1] += v.y * f; acc[4 * e + 2] += v.z * f; acc[4 * e + 3] += v.w * f;
+    }
+  }
+  if (b2 != -INFINITY) {
+    const float f = exp2f(b2 - m);
+    l += f;
+    const float* more = p.o_more + orow * kHeadDim + blockIdx.y * 16;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = fmaf(more[e], f, acc[e]);
+  }
+  const float inv = l > 0.f ? 1.f / l : (l != l ? l : 0.f);
+  uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + orow * kHeadDim * (p.out_dtype == 4 ? 4 : 2);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = acc[8 * k + e] * inv;
+    store_row16(dst, p.out_dtype, blockIdx.y * 2 + k, v);
+  }
+  if (p.lse && blockIdx.y == 0)
+    p.lse[orow] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : (l != l ? l : -INFINITY);
+}
+
+}  // namespace pkv

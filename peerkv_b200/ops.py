@@ -313,3 +313,287 @@ def quantize_kv(x: torch.Tensor, fmt: str) -> Tuple[torch.Tensor, torch.Tensor]:
     check(_lib.lib().pkv_quantize_kv(x.device.index, x.data_ptr(), _DT[x.dtype], rows, codes.data_ptr(),
                                      scales.data_ptr(), _DT[code_dt], _stream(x.device)))
     return codes, scales
+
+
+# --------------------------------------------------------------------------- #
+# prompts, shared prefixes, and the append in front of them
+# --------------------------------------------------------------------------- #
+_workspace_bytes = {}
+
+
+def _prompt_workspace(device: torch.device) -> torch.Tensor:
+    """Workspace of one pkv_prompt_attention call, from torch's allocator: it belongs to the
+    current stream (or to the graph being captured), so calls on other streams and other
+    captured graphs have their own."""
+    n = _workspace_bytes.get(device.index)
+    if n is None:
+        v = C.c_int64()
+        check(_lib.lib().pkv_prompt_workspace(device.index, C.byref(v)))
+        n = _workspace_bytes[device.index] = int(v.value)
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def _rows_of_heads(t: torch.Tensor, name: str) -> torch.Tensor:
+    """[tokens, heads, 128] as the kernels read it: unit last stride, the others positive
+    multiples of 8 elements, 16-byte aligned; anything else is copied."""
+    if t.dim() != 3 or t.shape[2] != HEAD_DIM:
+        raise PeerKVError(f"{name} must be [tokens, heads, {HEAD_DIM}]; got {tuple(t.shape)}")
+    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and \
+        all(n <= 1 or (st > 0 and st % 8 == 0) for n, st in zip(t.shape[:2], t.stride()[:2]))
+    return t if ok or t.numel() == 0 else t.contiguous()
+
+
+def _status_word(status: Optional[torch.Tensor], device: torch.device):
+    if status is None:
+        return None
+    if status.device != device or status.dtype != torch.int32 or status.numel() < 1:
+        raise PeerKVError("status must be an int32 tensor on the call's GPU")
+    return status.data_ptr()
+
+
+def _check_out(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out.shape != q.shape or out.device != q.device or not out.is_contiguous() or \
+            out.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise PeerKVError("out must be a contiguous fp16 / bf16 / fp32 tensor of q's shape on q's GPU")
+    return out
+
+
+def _prompt_call(q, view, scale, causal, out, lse, cu_q, n_seqs, status, block_table=None, seq_lens=None, cu_k=None,
+                 more=None):
+    a = _lib.PromptArgs()
+    a.q, a.q_token_stride, a.q_head_stride = q.data_ptr(), q.stride(0), q.stride(1)
+    a.dtype, a.n_q_heads, a.total_q, a.n_seqs = _DT[q.dtype], q.shape[1], q.shape[0], n_seqs
+    a.cu_seqlens_q = cu_q.data_ptr()
+    a.kv = view
+    if block_table is not None:
+        a.block_table, a.block_table_stride, a.block_table_cols = \
+            block_table.data_ptr(), block_table.stride(0), block_table.shape[1]
+        a.seq_lens = seq_lens.data_ptr()
+    else:
+        a.cu_seqlens_k = cu_k.data_ptr()
+    if more is not None:
+        a.o_more, a.lse_more = more[0].data_ptr(), more[1].data_ptr()
+    a.scale, a.causal = float(scale), 1 if causal else 0
+    ws = _prompt_workspace(q.device)
+    check(_lib.lib().pkv_prompt_attention(q.device.index, C.byref(a), out.data_ptr(), _DT[out.dtype],
+                                          lse.data_ptr() if lse is not None else None, ws.data_ptr(), ws.numel(),
+                                          _status_word(status, q.device), _stream(q.device)))
+
+
+def _check_prompt_q(q: torch.Tensor) -> torch.Tensor:
+    _require_cuda(q, "q")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise PeerKVError(f"q must be fp16 or bf16; got {q.dtype}")
+    return _rows_of_heads(q, "q")
+
+
+def _cu(t, device, name) -> torch.Tensor:
+    t = _meta(t, device, name)
+    if t.dim() != 1 or t.numel() < 1:
+        raise PeerKVError(f"{name} must be [n_seqs + 1]")
+    return t
+
+
+def _prompt_pool(q, k_pool, v_pool):
+    for t, n in ((k_pool, "k_pool"), (v_pool, "v_pool")):
+        _same_gpu(t, q.device, n)
+    view = paged_view(k_pool, v_pool)
+    if k_pool.dtype != q.dtype or v_pool.dtype != q.dtype:
+        raise PeerKVError(f"k_pool ({k_pool.dtype}), v_pool ({v_pool.dtype}) and q ({q.dtype}) must share a dtype")
+    return view
+
+
+def _table(block_table, device, rows: int, name: str) -> torch.Tensor:
+    bt = _meta(block_table, device, name)
+    if bt.dim() != 2 or bt.shape[0] != rows:
+        raise PeerKVError(f"{name} must be [{rows}, pages]; got {tuple(bt.shape)}")
+    return bt if bt.shape[1] > 0 else bt.new_zeros(rows, 1)
+
+
+def prefill_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
+                  seq_lens: torch.Tensor, cu_seqlens_q: torch.Tensor, scale: Optional[float] = None, causal: bool = True,
+                  out: Optional[torch.Tensor] = None, return_lse: bool = False,
+                  status: Optional[torch.Tensor] = None):
+    """Attention of whole prompts, chunks or single new tokens over the paged cache of one GPU.
+
+    q [total_q, Hq, 128] fp16 / bf16, the new tokens of all sequences one behind the other:
+    sequence i owns rows cu_seqlens_q[i] .. cu_seqlens_q[i+1] - 1 (possibly none).  seq_lens [n]
+    counts every token of a sequence in the cache, the new ones included: append them first
+    (norm_rope_append).  k_pool / v_pool, block_table as in decode_paged, 16-bit, page size a
+    multiple of 16.  With `causal` row r of n new ones sees keys j <= seq_len - n + r.
+    Returns out [total_q, Hq, 128] (q's dtype, or `out`'s), and with return_lse the natural-log lse
+    [total_q, Hq] fp32, so that shards merge with merge_partials.  Rows that see nothing are 0 with
+    lse -inf; rows behind the last sequence are not written.  V of every token of a sequence
+    must be finite; what the pages hold behind a sequence does not matter.
+    `status` (int32 [1] on q's GPU) gets the device status bits OR-ed in."""
+    q = _check_prompt_q(q)
+    cu = _cu(cu_seqlens_q, q.device, "cu_seqlens_q")
+    n = cu.numel() - 1
+    bt = _table(block_table, q.device, n, "block_table")
+    sl = _meta(seq_lens, q.device, "seq_lens")
+    if sl.dim() != 1 or sl.numel() != n:
+        raise PeerKVError(f"seq_lens must be [{n}]; got {tuple(sl.shape)}")
+    view = _prompt_pool(q, k_pool, v_pool)
+    out = _check_out(out, q)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+    _prompt_call(q, view, 1.0 / math.sqrt(HEAD_DIM) if scale is None else scale, causal, out, lse, cu, n, status,
+                 block_table=bt, seq_lens=sl)
+    return (out, lse) if return_lse else out
+
+
+def prefill_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                   cu_seqlens_k: Optional[torch.Tensor] = None, scale: Optional[float] = None, causal: bool = True,
+                   out: Optional[torch.Tensor] = None, return_lse: bool = False,
+                   status: Optional[torch.Tensor] = None):
+    """prefill_paged for keys that are packed like the queries: k, v [total_k, Hkv, 128] (views
+    into the fused projection are fine), sequence i owns keys cu_seqlens_k[i] ..
+    cu_seqlens_k[i+1] - 1 (default: the queries' offsets)."""
+    q = _check_prompt_q(q)
+    _same_gpu(k, q.device, "k"); _same_gpu(v, q.device, "v")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise PeerKVError(f"k ({k.dtype}), v ({v.dtype}) and q ({q.dtype}) must share a dtype")
+    if k.shape != v.shape:
+        raise PeerKVError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must have one shape")
+    k, v = _rows_of_heads(k, "k"), _rows_of_heads(v, "v")
+    if k.stride() != v.stride():
+        k, v = k.contiguous(), v.contiguous()
+    cu = _cu(cu_seqlens_q, q.device, "cu_seqlens_q")
+    ck = cu if cu_seqlens_k is None else _cu(cu_seqlens_k, q.device, "cu_seqlens_k")
+    if ck.numel() != cu.numel():
+        raise PeerKVError("cu_seqlens_q and cu_seqlens_k must describe the same number of sequences")
+    view = KvView()
+    view.k, view.v = k.data_ptr(), v.data_ptr()
+    view.dtype, view.n_kv_heads, view.head_dim = _DT[k.dtype], k.shape[1], HEAD_DIM
+    view.page_size, view.n_pages = k.shape[0], 1 if k.shape[0] > 0 else 0
+    view.token_stride, view.head_stride, view.page_stride = k.stride(0), k.stride(1), HEAD_DIM
+    out = _check_out(out, q)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
+    _prompt_call(q, view, 1.0 / math.sqrt(HEAD_DIM) if scale is None else scale, causal, out, lse, cu, cu.numel() - 1,
+                 status, cu_k=ck)
+    return (out, lse) if return_lse else out
+
+
+def decode_shared_prefix(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, prefix_table: torch.Tensor,
+                         prefix_lens: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                         group_offsets: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                         out: Optional[torch.Tensor] = None, return_lse: bool = False, shard: Optional[Shard] = None,
+                         status: Optional[torch.Tensor] = None):
+    """Decode attention (one token per sequence) of groups of sequences that share a prefix: the
+    prefix is read once for its group instead of once per sequence.
+
+    q [batch, Hq, 128]; group g owns sequences group_offsets[g] .. group_offsets[g+1] - 1 (default:
+    one group of all; the offsets run from 0 to batch) and the prefix of prefix_lens[g]
+    tokens in the pages prefix_table[g] (any length, 0 allowed).  block_table / seq_lens
+    describe what each sequence has of its own behind the prefix (0 tokens allowed), e.g.
+    the columns of a full table behind the shared pages.  Result as decode_paged over prefix
+    and own tokens: out [batch, Hq, 128], with return_lse the lse [batch, Hq].
+    The own tokens go through `shard` (see decode_paged), whose launches must not overlap."""
+    q = _check_prompt_q(q)
+    B, Hq, D = q.shape
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+    pt = prefix_table if prefix_table.dim() == 2 else prefix_table[None]
+    go = torch.tensor([0, B], dtype=torch.int32, device=q.device) if group_offsets is None \
+        else _cu(group_offsets, q.device, "group_offsets")
+    n = go.numel() - 1
+    pt = _table(pt, q.device, n, "prefix_table")
+    pl = _meta(prefix_lens, q.device, "prefix_lens").reshape(-1)
+    if pl.numel() != n:
+        raise PeerKVError(f"prefix_lens must be [{n}]; got {pl.numel()} of them")
+    bt, sl = _table(block_table, q.device, B, "block_table"), _meta(seq_lens, q.device, "seq_lens")
+    if sl.dim() != 1 or sl.numel() != B:
+        raise PeerKVError(f"seq_lens must be [{B}]; got {tuple(sl.shape)}")
+    view = _prompt_pool(q, k_pool, v_pool)
+    out = _check_out(out, q)
+    lse = torch.empty(B, Hq, dtype=torch.float32, device=q.device) if return_lse else None
+    if B > 0:
+        own = partial_paged(q, k_pool, v_pool, bt, sl, scale, shard=shard)
+        _prompt_call(q, view, scale, False, out, lse, go, n, status, block_table=pt, seq_lens=pl, more=own)
+    return (out, lse) if return_lse else out
+
+
+def norm_rope_append(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optional[torch.Tensor], n_q_heads: int,
+                     n_kv_heads: int, q_out: Optional[torch.Tensor] = None, k_pool: Optional[torch.Tensor] = None,
+                     v_pool: Optional[torch.Tensor] = None, slot_mapping: Optional[torch.Tensor] = None, k_scale=None,
+                     v_scale=None, q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                     eps: float = 1e-6, interleaved: bool = False, gain: float = 1.0, peers=(), bases=(),
+                     status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """New tokens on their way into the cache, one launch: per-head RMS norm of q and k (where
+    q_weight / k_weight [128] are given), rotary positions, and the store of k and v by slot.
+
+    qkv [T, (Hq + 2 Hkv) * 128] fp16 / bf16 (rows may be strided); positions [T] int64; inv_freq
+    fp32 [rot / 2], which says how much of a head turns (rot a multiple of 16, at most 128;
+    None: no rotation), halves against each other or, with `interleaved`, neighbours; `gain`
+    multiplies cos and sin.  q goes to q_out [T, Hq, 128] (made if None; it may be the q part of qkv).
+    slot_mapping [T] int64 = page * page_size + offset (negative: not stored); the slots of one
+    call must differ.  k_pool / v_pool [n_pages, page, Hkv, 128] of qkv's dtype, int8 or
+    float8_e4m3fn with k_scale / v_scale [n_pages, page, Hkv] fp16; `peers` = further (k_pool,
+    v_pool[, k_scale, v_scale]) on other GPUs, holding the page ids from `bases` on.
+    Returns q_out.  A slot outside every pool is skipped and sets bit 2 in `status`."""
+    _require_cuda(qkv, "qkv")
+    dev = qkv.device
+    if qkv.dtype not in (torch.float16, torch.bfloat16):
+        raise PeerKVError(f"qkv must be fp16 or bf16; got {qkv.dtype}")
+    if qkv.dim() != 2 or n_q_heads < 1 or n_kv_heads < 1 or qkv.shape[1] != (n_q_heads + 2 * n_kv_heads) * HEAD_DIM:
+        raise PeerKVError(f"qkv must be [T, (n_q_heads + 2 n_kv_heads) * {HEAD_DIM}]; got {tuple(qkv.shape)}")
+    T = qkv.shape[0]
+    if T and (qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16):
+        qkv = qkv.contiguous()
+    if q_out is None:
+        q_out = torch.empty(T, n_q_heads, HEAD_DIM, dtype=qkv.dtype, device=dev)
+    if tuple(q_out.shape) != (T, n_q_heads, HEAD_DIM) or q_out.dtype != qkv.dtype or q_out.device != dev or \
+            (T and (q_out.stride(2) != 1 or (n_q_heads > 1 and q_out.stride(1) != HEAD_DIM))):
+        raise PeerKVError(f"q_out must be [T, n_q_heads, {HEAD_DIM}] of qkv's dtype and GPU with contiguous heads")
+
+    def vector(t, n, dt, name):
+        if t is None:
+            return None
+        if t.device != dev or t.dtype != dt or t.dim() != 1 or t.numel() != n:
+            raise PeerKVError(f"{name} must be {dt} [{n}] on {dev}; got {t.dtype} {tuple(t.shape)} on {t.device}")
+        return t if t.is_contiguous() else t.contiguous()
+
+    half = 0 if inv_freq is None else inv_freq.numel()
+    pos = positions if positions.dtype == torch.int64 else positions.to(torch.int64)
+    keep = [qkv, vector(pos, T, torch.int64, "positions"), vector(inv_freq, half, torch.float32, "inv_freq"),
+            vector(q_weight, HEAD_DIM, qkv.dtype, "q_weight"), vector(k_weight, HEAD_DIM, qkv.dtype, "k_weight")]
+    a = _lib.AppendArgs()
+    a.qkv, a.qkv_stride = qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1]
+    a.positions, a.inv_freq, a.q_weight, a.k_weight = [t.data_ptr() if t is not None else None for t in keep[1:]]
+    a.q_out, a.q_out_stride = q_out.data_ptr(), q_out.stride(0) if T > 1 else n_q_heads * HEAD_DIM
+    a.n_tokens, a.n_q_heads, a.n_kv_heads, a.head_dim = T, n_q_heads, n_kv_heads, HEAD_DIM
+    a.dtype, a.rot_dim, a.interleaved = _DT[qkv.dtype], 2 * half, 1 if interleaved else 0
+    a.eps, a.gain = float(eps), float(gain)
+    if slot_mapping is not None:
+        if k_pool is None or v_pool is None:
+            raise PeerKVError("an append needs k_pool, v_pool and slot_mapping")
+        sm = slot_mapping if slot_mapping.dtype == torch.int64 else slot_mapping.to(torch.int64)
+        keep.append(vector(sm, T, torch.int64, "slot_mapping"))
+        a.slot_mapping = keep[-1].data_ptr()
+        pools = [(k_pool, v_pool, k_scale, v_scale)] + [tuple(p) + (None,) * (4 - len(p)) for p in peers]
+        if len(bases) != len(pools) - 1:
+            raise PeerKVError("every peer pool needs its first page id in bases")
+        _same_gpu(k_pool, dev, "k_pool")
+        views = (KvView * len(pools))()
+        for i, (kp, vp, ks, vs) in enumerate(pools):
+            for t in (vp, ks, vs):
+                _same_gpu(t, kp.device, f"pool {i}")
+            if kp.dtype != vp.dtype or kp.dtype not in (qkv.dtype, torch.int8, torch.float8_e4m3fn):
+                raise PeerKVError(f"pool {i}: {kp.dtype} / {vp.dtype}; qkv's dtype, int8 or float8_e4m3fn")
+            if kp.element_size() == 1:
+                for t in (ks, vs):
+                    if t is None or t.dtype != torch.float16 or t.shape != kp.shape[:3] or not t.is_contiguous():
+                        raise PeerKVError("quantised pools need contiguous fp16 k_scale / v_scale [n_pages, page, Hkv]")
+            if kp.shape[2] != n_kv_heads or kp.shape[3] != HEAD_DIM:
+                raise PeerKVError(f"pool {i} must be [n_pages, page, {n_kv_heads}, {HEAD_DIM}]; got {tuple(kp.shape)}")
+            views[i] = paged_view(kp, vp, ks, vs)
+        if peers:
+            from .peerkv.kv_alloc import _enable_peer_access
+            _enable_peer_access(dev, [p[0].device for p in pools[1:]])
+        a.pools, a.n_dev = views, len(pools)
+        first = (C.c_int64 * len(pools))(0, *[int(b) for b in bases])
+        a.bases = first
+    elif k_pool is not None or v_pool is not None:
+        raise PeerKVError("an append needs k_pool, v_pool and slot_mapping")
+    check(_lib.lib().pkv_norm_rope_append(dev.index, C.byref(a), _status_word(status, dev), _stream(dev)))
+    return q_out

@@ -1,0 +1,158 @@
+"""The work split of the prompt-attention kernel, restated on the host: every KV tile of every
+item is done exactly once, a CTA's pieces never share a workspace slot, the join finds exactly
+the pieces that were written, and the ring of K / V tiles is filled in the order in which the
+matrix-instruction warp reads it."""
+import os
+import random
+import re
+
+import pytest
+
+SRC = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "peerkv_b200", "csrc",
+                        "prompt_kernel.cuh")).read()
+
+
+def const(name):
+    return int(re.search(r"constexpr int %s = (\d+)" % name, SRC).group(1))
+
+
+ITEM_COST, MIN_PIECE, KEYS, ROWS, SLOTS = (const(n) for n in ("kPaItemCost", "kPaMinPiece", "kPaKeys", "kPaRows",
+                                                              "kPaSlots"))
+
+
+def items(seqs, hkv, group, causal):
+    """(name on the cost axis, cost, KV tiles, tokens) of every item in order."""
+    tt, a, out = 2 * (ROWS // group), 0, []
+    for n, length in seqs:
+        tiles = -(-n // tt)
+        for _ in range(hkv):
+            for t in range(tiles):
+                cost = (max(length - n, 0) if causal else length) + ITEM_COST + (tt * (t + 1) if causal else 0)
+                n_tok = min(tt, n - t * tt)
+                vis = max(0, min(length, length - n + t * tt + n_tok)) if causal else length
+                out.append((a, cost, -(-vis // KEYS), n_tok))
+                a += cost
+    return out, a
+
+
+def cut(y, cost, n):
+    return 0 if y <= 0 else n if y >= cost else y * n // cost
+
+
+def pieces(its, total, grid):
+    """Per CTA: list of (item index, kt0, kt1, slot or None when written directly), and its record."""
+    n_cta = min(grid, -(-total // MIN_PIECE))
+    work, rec = [], []
+    for c in range(n_cta):
+        x0, x1 = total * c // n_cta, total * (c + 1) // n_cta
+        assert x1 > x0
+        mine, first = [], None
+        for i, (a, cost, n, _) in enumerate(its):
+            if a + cost <= x0 or a >= x1:
+                continue
+            k0, k1 = cut(x0 - a, cost, n), cut(x1 - a, cost, n)
+            if first is None:
+                first = (i, x0 > a, k0, k1, n)
+            if k1 > k0 or (n == 0 and x0 <= a):
+                whole = k0 == 0 and k1 == n
+                mine.append((i, k0, k1, None if whole else 2 * c + (0 if x0 > a else 1)))
+        work.append(mine)
+        rec.append(first)
+    return work, rec
+
+
+def join(rec, c):
+    """Slots block c adds up and the item, or None."""
+    i, mid, k0, k1, n = rec[c]
+    if not mid or k0 >= n or (c > 1 and rec[c - 1][1] and rec[c - 1][0] == i) or (k0 == 0 and k1 == n):
+        return None
+    last = c
+    while last + 1 < len(rec):
+        j, jmid, j0, j1, jn = rec[last + 1]
+        if not jmid or j != i:
+            break
+        if j0 == 0 and j1 == jn:
+            return None
+        last += 1
+    slots = [2 * (c - 1) + 1] if k0 > 0 else []
+    return i, slots + [2 * d for d in range(c, last + 1) if rec[d][3] > rec[d][2]]
+
+
+def check(seqs, hkv, group, causal, grid):
+    its, total = items(seqs, hkv, group, causal)
+    if total == 0:
+        return
+    work, rec = pieces(its, total, grid)
+    done = {i: [] for i in range(len(its))}
+    written = {}
+    for c, mine in enumerate(work):
+        slots = [s for *_, s in mine if s is not None]
+        assert len(set(slots)) == len(slots)
+        for i, k0, k1, s in mine:
+            done[i].append((k0, k1))
+            if s is not None:
+                written.setdefault(i, []).append(s)
+    for i, (_, _, n, _) in enumerate(its):
+        at = 0
+        for k0, k1 in done[i]:
+            assert k0 == at
+            at = k1
+        assert at == n and done[i], (i, n, done[i])
+    joined = {}
+    for c in range(1, len(rec)):
+        j = join(rec, c)
+        if j is not None:
+            assert j[0] not in joined
+            joined[j[0]] = j[1]
+    assert {i: sorted(s) for i, s in joined.items()} == {i: sorted(s) for i, s in written.items()}
+    assert all(len(s) > 1 for s in joined.values())
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_every_tile_once(seed):
+    rng = random.Random(seed)
+    seqs = []
+    for _ in range(rng.choice([1, 1, 2, 5, 20])):
+        n = rng.choice([0, 1, 1, 2, 63, 64, 65, rng.randint(1, 3000)])
+        seqs.append((n, rng.choice([0, n, n // 2, n + rng.randint(0, 20000)])))
+    check(seqs, rng.choice([1, 2, 8]), rng.choice([1, 3, 4, 8, 128]), rng.random() < 0.6, rng.choice([1, 7, 148]))
+
+
+def test_edge_lengths():
+    for n, length in [(1, 1), (1, 0), (3, 0), (64, 1), (300, 7), (1, 1 << 20), (4, 2048), (257, 257)]:
+        for causal in (False, True):
+            check([(n, length)], 8, 4, causal, 148)
+
+
+def ring_order(n_tiles, two):
+    """Order in which the load warp fills the ring."""
+    if two:
+        return [x for j in range(n_tiles) for x in (("K", j), ("V", j))]
+    out = [("K", 0)] + ([("K", 1)] if n_tiles > 1 else [])
+    for i in range(n_tiles):
+        out.append(("V", i))
+        if i + 2 < n_tiles:
+            out.append(("K", i + 2))
+    return out
+
+
+@pytest.mark.parametrize("n_tiles", [1, 2, 3, 4, 5, 6, 17])
+def test_ring_positions(n_tiles):
+    """The positions the matrix-instruction warp computes, and that no load waits for a slot whose
+    release needs a later load."""
+    order = ring_order(n_tiles, False)
+    k_at = lambda i: i if i < 2 else 2 * i - 1
+    v_at = lambda i: 2 * i + 2 if i + 1 < n_tiles else 2 * i + 1
+    for i in range(n_tiles):
+        assert order[k_at(i)] == ("K", i) and order[v_at(i)] == ("V", i)
+    for two in (False, True):
+        order = ring_order(n_tiles, two)
+        # reads in program order of the issuing warp; a read releases its slot
+        reads = [("K", 0)] if two else [("K", i) for i in range(min(2, n_tiles))]
+        for i in range(n_tiles):
+            if two:
+                reads += [("V", i)] + ([("K", i + 1)] if i + 1 < n_tiles else [])
+            else:
+                reads += [("V", i)] + ([("K", i + 2)] if i + 2 < n_tiles else [])
+        for step, r in enumerate(reads):
+            assert order.index(r) <= step + SLOTS - 1
