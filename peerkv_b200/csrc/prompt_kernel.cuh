@@ -14,7 +14,7 @@
 // alternate KV tiles instead and joins their accumulators at the end.
 //
 // Warps (384 threads, one CTA per SM): 0-3 and 4-7 the two softmax warpgroups, one thread per
-// row; 8 issues the TMA loads; 9 issues the tcgen05 instructions; 10-11 idle.
+// row; 8 issues the TMA loads; 9 issues the tcgen05 instructions; 10 walks the work list; 11 idle.
 // TMEM: S0 S1 O0 O1, 128 columns each; the 16-bit P overwrites the first half of its S.
 // Shared memory: Q 2 x 32 KB, a ring of five 32 KB slots that K and V tiles of 128 keys take
 // turns in (K0 V0 K1 V1 ..., the order in which the products need them).
@@ -44,10 +44,13 @@ constexpr int kPaTileBytes = kPaKeys * kHeadDim * 2;     // 32 KB
 constexpr int kPaHalfBytes = kPaTileBytes / 2;           // 128 rows x 64 values, 128-byte swizzle
 constexpr int kPaRingOff = 2 * kPaTileBytes;
 constexpr int kPaMiscOff = kPaRingOff + kPaSlots * kPaTileBytes;
-constexpr int kPaMiscBytes = 512 + 128 * 8;
+constexpr int kPaMiscBytes = 640 + 128 * 8;
 constexpr int kPaSmem = kPaMiscOff + kPaMiscBytes + 1024;  // 1 KB to align the base
 static_assert(kPaSmem <= 232448, "shared memory of a CTA");
 constexpr int kPaMaxCtas = 256;
+// 384 threads x 168 registers at launch = 64512; 256 x 208 + 128 x 80 = 63488 after the split.
+constexpr int kPaSoftmaxRegs = 208;
+constexpr int kPaOtherRegs = 80;
 constexpr uint32_t kPaColO = 256;                        // TMEM columns: S0 0, S1 128, O0 256, O1 384
 constexpr int kPaItemCost = 192;   // what an item costs besides its keys, in keys
 constexpr int kPaMinPiece = 512;   // no CTA gets less than this many keys of work
@@ -175,6 +178,18 @@ struct PromptItem {
   __device__ __forceinline__ bool two(const PromptParams& p) const { return n_tok > p.tok_tile; }
 };
 
+// What the other warps need of an item: the scheduling warp hands it to them through shared
+// memory, so that the cost axis and its 64-bit arithmetic live in one warp's registers.
+struct __align__(16) PromptWork {
+  int n_tiles;                 // KV tiles of this CTA's share; -1: no more items
+  int kt0, vis, len;           // first tile; keys the item's last row sees; the sequence's keys
+  int lim0;                    // keys token 0 of the item sees (causal), or len
+  int q0, n_tok, h;            // first packed row, tokens, kv-head
+  int s, k0;                   // sequence; first packed key
+  int two, slot;               // two row tiles; workspace slot, or -1: written directly
+};
+constexpr int kPaWorkRing = 4;
+
 // ---- bounded waits -------------------------------------------------------------------- //
 // A step of the pipeline takes microseconds; a wait that has not ended after two seconds sets
 // the abort flag, every later wait returns at once, and the CTA runs out.
@@ -224,17 +239,21 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   auto p_full = [&](int w) { return bars + 8u * (15 + w); };
   auto o_full = [&](int w) { return bars + 8u * (17 + w); };
   const uint32_t x_ready = bars + 8u * 19, x_done = bars + 8u * 20;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 192);
-  uint32_t* tmem_word = reinterpret_cast<uint32_t*>(misc + 196);
-  volatile int64_t* first = reinterpret_cast<volatile int64_t*>(misc + 208);   // s, base, total
-  int64_t* wsum = reinterpret_cast<int64_t*>(misc + 256);                      // 12 warp sums
-  float2* xml = reinterpret_cast<float2*>(misc + 512);                         // [128] (m, l) of stream 1
+  auto w_full = [&](uint32_t i) { return bars + 8u * (21 + i % kPaWorkRing); };
+  auto w_empty = [&](uint32_t i) { return bars + 8u * (21 + kPaWorkRing + i % kPaWorkRing); };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 240);
+  uint32_t* tmem_word = reinterpret_cast<uint32_t*>(misc + 244);
+  volatile int64_t* first = reinterpret_cast<volatile int64_t*>(misc + 256);   // s, base
+  int64_t* wsum = reinterpret_cast<int64_t*>(misc + 272);                      // 12 warp sums
+  PromptWork* ring = reinterpret_cast<PromptWork*>(misc + 384);                // 4 x 48 bytes
+  float2* xml = reinterpret_cast<float2*>(misc + 640);                         // [128] (m, l) of stream 1
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kPaSlots; ++i) { mbar_init(full(i), 1); mbar_init(empty(i), 1); }
     mbar_init(q_full, 1); mbar_init(q_empty, 1); mbar_init(done, 1);
     for (int w = 0; w < 2; ++w) { mbar_init(s_full(w), 1); mbar_init(p_full(w), 4); mbar_init(o_full(w), 1); }
     mbar_init(x_ready, 4); mbar_init(x_done, 4);
+    for (int i = 0; i < kPaWorkRing; ++i) { mbar_init(w_full(i), 1); mbar_init(w_empty(i), 10); }
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -269,15 +288,13 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   }
   const int n_cta = (int)min((int64_t)gridDim.x, (total + kPaMinPiece - 1) / kPaMinPiece);
   const bool active = (int)blockIdx.x < n_cta;
-  PromptItem it;
-  it.x0 = active ? total * blockIdx.x / n_cta : 0;
-  it.x1 = active ? total * (blockIdx.x + 1) / n_cta : 0;
-  if (active && before <= it.x0 && it.x0 < before + mine) {
+  const int64_t x0 = active ? total * blockIdx.x / n_cta : 0, x1 = active ? total * (blockIdx.x + 1) / n_cta : 0;
+  if (active && before <= x0 && x0 < before + mine) {
     int64_t base = before;
     for (int s = sb; s < se; ++s) {
       const PromptSeq q = prompt_seq(p, s);
       const int64_t c = p.n_kv_heads * prompt_items_cost(q, q.tiles);
-      if (it.x0 < base + c) { first[0] = s; first[1] = base; break; }
+      if (x0 < base + c) { first[0] = s; first[1] = base; break; }
       base += c;
     }
   }
@@ -285,37 +302,37 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   __syncthreads();
   const uint32_t tmem = *tmem_word;
 
-  if (active) {
-    it.s = (int)first[0];
-    it.start(p, first[1]);
-    if (threadIdx.x == 0) {
-      PromptRec r;
-      r.a = it.a; r.mid = it.x0 > it.a ? 1 : 0; r.kt0 = it.kt0; r.kt1 = it.kt1; r.n = it.n;
-      r.q0 = it.q0; r.n_tok = it.n_tok; r.h = it.h; r.pad = 0;
-      p.rec[blockIdx.x] = r;
-    }
-  }
-
-  if (active && warp < 8) {
+  // Every reader warp takes the items in turn: wait, copy, give the place back.
+  uint32_t n_work = 0;
+  PromptWork wk;
+  auto take = [&]() {
+    if (!pa_wait(w_full(n_work), (n_work / kPaWorkRing) & 1, abort_flag)) return false;
+    wk = ring[n_work % kPaWorkRing];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(w_empty(n_work));
+    ++n_work;
+    return wk.n_tiles >= 0;
+  };
+  if (warp < 8) {
     // ------------------------------ softmax warpgroups ------------------------------ //
+    setmaxnreg_inc<kPaSoftmaxRegs>();
     const int w = warp >> 2, row = threadIdx.x & 127;
     const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);      // lane 32 * (warp % 4)
     const uint32_t ts = lane_base + w * 128, to = lane_base + kPaColO + w * 128;
-    const int tok_in = row / p.group, head_in = row - tok_in * p.group;
+    const int tok_in = row / p.group;
     const float sl = p.scale_log2;
     uint32_t n_s = 0, n_o = 0, n_x = 0;                                   // barrier phases used
-    bool ok = true;
-    do {
-      if (!it.mine()) continue;
-      const bool two = it.two(p);
+    while (active && take()) {
+      const bool two = wk.two;
       const int tok = (two ? w * p.tok_tile : 0) + tok_in;               // token of this row in the item
-      const int n_tiles = it.kt1 - it.kt0;
-      const int steps = two ? n_tiles : (n_tiles + 1 - w) >> 1;          // one row tile: alternate KV tiles
+      const int steps = two ? wk.n_tiles : (wk.n_tiles + 1 - w) >> 1;    // one row tile: alternate KV tiles
       // keys [0, lim) are visible to this row
-      const int lim = p.causal ? min(it.seq.len, it.seq.len - it.seq.n + (it.q0 - it.seq.q0) + tok + 1) : it.seq.len;
+      const int lim = p.causal ? min(wk.len, wk.lim0 + tok) : wk.len;
+      int left = lim - (wk.kt0 + (two ? 0 : w)) * kPaKeys;               // of them, in and behind this tile
+      const int stride = two ? kPaKeys : 2 * kPaKeys;
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < steps; ++j) {
-        const int key0 = (it.kt0 + (two ? j : 2 * j + w)) * kPaKeys;
+      bool ok = true;
+      for (int j = 0; j < steps; ++j, left -= stride) {
         if (!(ok = pa_wait(s_full(w), n_s & 1, abort_flag))) break;
         ++n_s;
         tc_fence_after();
@@ -323,8 +340,7 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(sreg[c], ts + c * 32);
         tmem_wait_ld();
-        if (__any_sync(0xffffffffu, key0 + kPaKeys > lim)) {
-          const int left = lim - key0;
+        if (__any_sync(0xffffffffu, left < kPaKeys)) {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -334,9 +350,10 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         float mx[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          mx[c] = __uint_as_float(sreg[c][0]);
+          mx[c] = fmaxf(__uint_as_float(sreg[c][0]), __uint_as_float(sreg[c][1]));
 #pragma unroll
-          for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(sreg[c][i]));
+          for (int i = 2; i < 32; i += 2)
+            mx[c] = max3(mx[c], __uint_as_float(sreg[c][i]), __uint_as_float(sreg[c][i + 1]));
         }
         const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         if (j == 0) {
@@ -349,38 +366,40 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           l *= alpha;
           m = mn;
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t o[32];
-            tmem_ld32(o, to + c * 32);
+          for (int c = 0; c < 8; ++c) {
+            uint32_t o[16];
+            tmem_ld16(o, to + c * 16);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            tmem_st32(to + c * 32, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st16(to + c * 16, o);
           }
         }
         // a row that has seen no key yet has m = -inf: 0 as the reference keeps exp2(-inf) = 0
         const float ref = m == -INFINITY ? 0.f : -m * sl;
-        float sum0 = 0.f, sum1 = 0.f, sum2 = 0.f, sum3 = 0.f;
+        const uint64_t sl2 = pack_f32x2(sl, sl), ref2 = pack_f32x2(ref, ref);
+        uint64_t sum_a = 0, sum_b = 0;                                     // two fp32 sums each
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            const float e0 = fast_exp2(fmaf(__uint_as_float(sreg[c][i]), sl, ref));
-            const float e1 = fast_exp2(fmaf(__uint_as_float(sreg[c][i + 1]), sl, ref));
-            const float e2 = fast_exp2(fmaf(__uint_as_float(sreg[c][i + 2]), sl, ref));
-            const float e3 = fast_exp2(fmaf(__uint_as_float(sreg[c][i + 3]), sl, ref));
-            sum0 += e0; sum1 += e1; sum2 += e2; sum3 += e3;
+            const float2 x = unpack_f32x2(fma_f32x2(pack_u32x2(sreg[c][i], sreg[c][i + 1]), sl2, ref2));
+            const float2 y = unpack_f32x2(fma_f32x2(pack_u32x2(sreg[c][i + 2], sreg[c][i + 3]), sl2, ref2));
+            const float e0 = fast_exp2(x.x), e1 = fast_exp2(x.y), e2 = fast_exp2(y.x), e3 = fast_exp2(y.y);
+            sum_a = add_f32x2(sum_a, pack_f32x2(e0, e1));
+            sum_b = add_f32x2(sum_b, pack_f32x2(e2, e3));
             pk[i / 2] = pack2<BF16>(e0, e1);
             pk[i / 2 + 1] = pack2<BF16>(e2, e3);
           }
           tmem_st16(ts + c * 16, pk);
         }
-        l += (sum0 + sum1) + (sum2 + sum3);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full(w));
+        const float2 sa = unpack_f32x2(add_f32x2(sum_a, sum_b));
+        l += sa.x + sa.y;
       }
       if (!ok) break;
 
@@ -388,20 +407,20 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       float a0 = 1.f, a1 = 0.f;                 // weights of O_w and (one row tile) of the other stream's O
       bool join = false;
       if (steps > 0) {
-        if (!(ok = pa_wait(o_full(w), n_o & 1, abort_flag))) break;
+        if (!pa_wait(o_full(w), n_o & 1, abort_flag)) break;
         ++n_o;
         tc_fence_after();
       }
-      if (!two && n_tiles > 1) {
+      if (!two && wk.n_tiles > 1) {
         if (w == 1) {
           xml[row] = make_float2(m, l);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(x_ready);
-          if (!(ok = pa_wait(x_done, n_x & 1, abort_flag))) break;   // O1 and xml are free again
+          if (!pa_wait(x_done, n_x & 1, abort_flag)) break;          // O1 and xml are free again
           ++n_x;
         } else {
-          if (!(ok = pa_wait(x_ready, n_x & 1, abort_flag))) break;
+          if (!pa_wait(x_ready, n_x & 1, abort_flag)) break;
           ++n_x;
           tc_fence_after();
           const float2 other = xml[row];
@@ -414,9 +433,9 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         }
       }
       if (two || w == 0) {
-        const bool valid = tok < it.n_tok && row < p.tok_tile * p.group;
-        const bool whole = it.whole();
-        const int64_t orow = (int64_t)(it.q0 + tok) * p.n_q_heads + it.h * p.group + head_in;
+        const bool valid = tok < wk.n_tok && row < p.tok_tile * p.group;
+        const bool whole = wk.slot < 0;
+        const int64_t orow = (int64_t)(wk.q0 + tok) * p.n_q_heads + wk.h * p.group + (row - tok_in * p.group);
         const float m2 = m == -INFINITY ? -INFINITY : m * sl;           // base-2 units
         float wa = l > 0.f ? 1.f / l : 0.f, wb = 0.f;
         if (l != l) wa = l;                                            // NaN scores stay NaN
@@ -433,10 +452,9 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           }
           if (p.lse) p.lse[orow] = lse2 * 0.6931471805599453f;
         }
-        const int slot = 2 * blockIdx.x + (it.x0 > it.a ? 0 : 1);
         const int prow = (two ? w * kPaRows : 0) + row;
-        if (!whole) p.part_ml[(size_t)slot * 256 + prow] = make_float2(m2, l);
-        float4* po = p.part_o + (size_t)slot * 32 * 256 + prow;
+        if (!whole) p.part_ml[(size_t)wk.slot * 256 + prow] = make_float2(m2, l);
+        float4* po = p.part_o + (size_t)max(wk.slot, 0) * 32 * 256 + prow;
         uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + orow * kHeadDim * (p.out_dtype == 4 ? 4 : 2);
         const float* more = p.o_more ? p.o_more + orow * kHeadDim : nullptr;
 #pragma unroll 1
@@ -481,205 +499,251 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           if (lane == 0) mbar_arrive(x_done);
         }
       }
-    } while (it.next(p));
-  } else if (active && warp == 8) {
-    // ------------------------------------ loads ------------------------------------ //
-    const int boxes = kPaKeys / p.box_tok;              // of one half tile
-    const uint32_t box_bytes = (uint32_t)p.box_tok * 128u;
-    const bool paged = p.seq_lens != nullptr;
-    uint32_t n_tile = 0, n_q = 0;
-    bool ok = true;
-    do {
-      if (!it.mine() || it.kt1 == it.kt0) continue;
-      const bool two = it.two(p);
-      const int n_tiles = it.kt1 - it.kt0;
-      // Q: the group's heads of up to 2 * tok_tile tokens, in two halves of 64 values
-      if (!(ok = pa_wait(q_empty, (n_q & 1) ^ 1, abort_flag))) break;
-      ++n_q;
-      if (lane == 0) {
-        const uint32_t half = (uint32_t)p.tok_tile * p.group * 128u;
-        mbar_arrive_expect_tx(q_full, half * (two ? 4u : 2u));
-        for (int w = 0; w < (two ? 2 : 1); ++w)
-          for (int d = 0; d < 2; ++d)
-            tma_load_3d(smem + w * kPaTileBytes + d * kPaHalfBytes, &qmap, q_full, d * 64, it.h * p.group,
-                        it.q0 + w * p.tok_tile);
-      }
-      __syncwarp();
-      const int32_t* row = paged ? p.block_table + (int64_t)it.s * p.bt_stride : nullptr;
-      // one tile of K (kv = 0) or V (kv = 1): lane = 2 * box + half
-      auto load = [&](int kt, int kv) {
-        const int slot = n_tile % kPaSlots;
-        if (!pa_wait(empty(slot), ((n_tile / kPaSlots) & 1) ^ 1, abort_flag)) return false;
-        ++n_tile;
-        const int key0 = kt * kPaKeys;
-        const int n_box = min(boxes, (it.vis - key0 + p.box_tok - 1) / p.box_tok);   // >= 1
-        const uint32_t dst0 = smem + kPaRingOff + slot * kPaTileBytes;
-        const CUtensorMap* map = kv ? &vmap : &kmap;
-        if (lane == 0) mbar_arrive_expect_tx(full(slot), n_box * 2 * box_bytes);
+    }
+  } else {
+    setmaxnreg_dec<kPaOtherRegs>();
+    if (warp == 8) {
+      // ------------------------------------ loads ------------------------------------ //
+      const int boxes = kPaKeys / p.box_tok;              // of one half tile
+      const uint32_t box_bytes = (uint32_t)p.box_tok * 128u;
+      const bool paged = p.seq_lens != nullptr;
+      uint32_t n_tile = 0, n_q = 0;
+      bool ok = true;
+      while (ok && active && take()) {
+        const int n_tiles = wk.n_tiles;
+        if (n_tiles == 0) continue;
+        // Q: the group's heads of up to 2 * tok_tile tokens, in two halves of 64 values
+        if (!(ok = pa_wait(q_empty, (n_q & 1) ^ 1, abort_flag))) break;
+        ++n_q;
+        if (lane == 0) {
+          const uint32_t half = (uint32_t)p.tok_tile * p.group * 128u;
+          mbar_arrive_expect_tx(q_full, half * (wk.two ? 4u : 2u));
+          for (int w = 0; w < (wk.two ? 2 : 1); ++w)
+            for (int d = 0; d < 2; ++d)
+              tma_load_3d(smem + w * kPaTileBytes + d * kPaHalfBytes, &qmap, q_full, d * 64, wk.h * p.group,
+                          wk.q0 + w * p.tok_tile);
+        }
         __syncwarp();
-        if (lane < 2 * n_box) {
-          const int b = lane >> 1, d = lane & 1;
-          const uint32_t dst = dst0 + d * kPaHalfBytes + b * box_bytes;
-          if (paged) {
-            const int key = key0 + b * p.box_tok, pg = key / p.page_size, tok = key - pg * p.page_size;
-            int page = row[pg];
-            if (page < 0 || page >= p.n_pages) {
-              if (p.status) atomicOr(p.status, kStBadPage);
-              page = 0;
+        const int32_t* row = paged ? p.block_table + (int64_t)wk.s * p.bt_stride : nullptr;
+        // one tile of K (kv = 0) or V (kv = 1): lane = 2 * box + half
+        auto load = [&](int i, int kv) {
+          const int slot = n_tile % kPaSlots;
+          if (!pa_wait(empty(slot), ((n_tile / kPaSlots) & 1) ^ 1, abort_flag)) return false;
+          ++n_tile;
+          const int key0 = (wk.kt0 + i) * kPaKeys;
+          const int n_box = min(boxes, (wk.vis - key0 + p.box_tok - 1) / p.box_tok);   // >= 1
+          const uint32_t dst0 = smem + kPaRingOff + slot * kPaTileBytes;
+          const CUtensorMap* map = kv ? &vmap : &kmap;
+          if (lane == 0) mbar_arrive_expect_tx(full(slot), n_box * 2 * box_bytes);
+          __syncwarp();
+          if (lane < 2 * n_box) {
+            const int b = lane >> 1, d = lane & 1;
+            const uint32_t dst = dst0 + d * kPaHalfBytes + b * box_bytes;
+            if (paged) {
+              const int key = key0 + b * p.box_tok, pg = key / p.page_size, tok = key - pg * p.page_size;
+              int page = row[pg];
+              if (page < 0 || page >= p.n_pages) {
+                if (p.status) atomicOr(p.status, kStBadPage);
+                page = 0;
+              }
+              if (p.head_major) tma_load_4d_keep(dst, map, full(slot), d * 64, tok, wk.h, page);
+              else              tma_load_4d_keep(dst, map, full(slot), d * 64, wk.h, tok, page);
+            } else {
+              tma_load_4d_keep(dst, map, full(slot), d * 64, wk.h, wk.k0 + key0, 0);
             }
-            if (p.head_major) tma_load_4d_keep(dst, map, full(slot), d * 64, tok, it.h, page);
-            else              tma_load_4d_keep(dst, map, full(slot), d * 64, it.h, tok, page);
+          }
+          __syncwarp();
+          return true;
+        };
+        if (wk.two) {
+          for (int i = 0; i < n_tiles && ok; ++i) ok = load(i, 0) && load(i, 1);
+        } else {
+          ok = load(0, 0) && (n_tiles < 2 || load(1, 0));
+          for (int i = 0; i < n_tiles && ok; ++i) ok = load(i, 1) && (i + 2 >= n_tiles || load(i + 2, 0));
+        }
+      }
+      if (*abort_flag) {   // give the copies in flight a bounded chance to land before the CTA goes away
+        for (uint32_t back = 1; back <= (uint32_t)kPaSlots && back <= n_tile; ++back) {
+          const uint32_t i = n_tile - back;
+          mbar_wait_bounded(full(i % kPaSlots), (i / kPaSlots) & 1, kPollLimit);
+        }
+        if (n_q) mbar_wait_bounded(q_full, (n_q - 1) & 1, kPollLimit);
+      }
+    } else if (warp == 9) {
+      // ------------------------------- matrix instructions ----------------------------- //
+      // The warp stays together; one elected lane issues.
+      constexpr uint32_t idesc_qk = umma_idesc(BF16, false, kPaRows, kPaKeys);
+      constexpr uint32_t idesc_pv = umma_idesc(BF16, true, kPaRows, kHeadDim);
+      uint32_t n_tile = 0, n_q = 0, n_p0 = 0, n_p1 = 0;
+      bool ok = true;
+      auto wait_tile = [&](uint32_t i) { return pa_wait(full(i % kPaSlots), (i / kPaSlots) & 1, abort_flag); };
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t q_lo = umma_desc_lo(smem, 16), ring_k = umma_desc_lo(smem + kPaRingOff, 16),
+                     ring_v = umma_desc_lo(smem + kPaRingOff, kPaHalfBytes);
+      constexpr uint32_t hi = umma_desc_hi(1024), tile16 = kPaTileBytes / 16, half16 = kPaHalfBytes / 16;
+      auto qk = [&](int w, int qtile, uint32_t i) {         // S_w = Q K^T
+        const uint32_t qa = q_lo + qtile * tile16, ka = ring_k + (i % kPaSlots) * tile16;
+        if (elect_one()) {
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            const uint32_t off = (ks >> 2) * half16 + (ks & 3) * 2;
+            umma_ss(tm + w * 128, qa + off, hi, ka + off, hi, idesc_qk, ks > 0 ? 1u : 0u);
+          }
+          umma_commit(s_full(w));
+        }
+        __syncwarp();
+      };
+      auto pv = [&](int w, uint32_t i, int ksteps, bool first_tile) {   // O_w (+)= P_w V
+        const uint32_t va = ring_v + (i % kPaSlots) * tile16, keep = first_tile ? 0u : 1u;
+        if (elect_one()) {
+          if (ksteps == 8) {
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks)
+              umma_ts(tm + kPaColO + w * 128, tm + w * 128 + ks * 8, va + ks * 128, hi, idesc_pv, ks > 0 ? 1u : keep);
           } else {
-            tma_load_4d_keep(dst, map, full(slot), d * 64, it.h, it.seq.k0 + key0, 0);
+            for (int ks = 0; ks < ksteps; ++ks)
+              umma_ts(tm + kPaColO + w * 128, tm + w * 128 + ks * 8, va + ks * 128, hi, idesc_pv, ks > 0 ? 1u : keep);
           }
         }
         __syncwarp();
+      };
+      // V rows of the last 16-key step that lie behind the sequence hold whatever the page holds:
+      // their weights are 0, but 0 * NaN is not, so they are cleared in shared memory.
+      auto clean = [&](uint32_t i, int kt, int ksteps) {
+        const int from = wk.len - kt * kPaKeys, to = ksteps * 16;
+        if (from >= to) return;
+        uint8_t* v = sgen + kPaRingOff + (i % kPaSlots) * kPaTileBytes;
+        for (int r = max(from, 0); r < to; ++r) {
+          *reinterpret_cast<uint32_t*>(v + r * 128 + lane * 4) = 0u;
+          *reinterpret_cast<uint32_t*>(v + kPaHalfBytes + r * 128 + lane * 4) = 0u;
+        }
+        fence_proxy_async();
+        __syncwarp();
+      };
+      auto steps_of = [&](int kt) { return min(8, (wk.vis - kt * kPaKeys + 15) >> 4); };
+      auto wait_p = [&](int w) {
+        const bool r = w ? pa_wait(p_full(1), n_p1 & 1, abort_flag) : pa_wait(p_full(0), n_p0 & 1, abort_flag);
+        if (w) ++n_p1; else ++n_p0;
+        if (r) tc_fence_after();
+        return r;
+      };
+      // (all commits from one thread: elect_one picks the same lane every time)
+      auto commit = [&](uint32_t bar) { if (elect_one()) umma_commit(bar); __syncwarp(); };
+      while (ok && active && take()) {
+        const int n_tiles = __shfl_sync(0xffffffffu, wk.n_tiles, 0);     // uniform, and known to be
+        if (n_tiles == 0) continue;
+        if (!(ok = pa_wait(q_full, n_q & 1, abort_flag))) break;
+        ++n_q;
+        if (wk.two) {
+          // ring order K0 V0 K1 V1 ...: tile j's K is entry base + 2j, its V base + 2j + 1
+          const uint32_t base = n_tile;
+          n_tile += 2 * n_tiles;
+          if (!(ok = wait_tile(base))) break;
+          qk(0, 0, base);
+          qk(1, 1, base);
+          commit(empty(base % kPaSlots));
+          if (n_tiles == 1) commit(q_empty);
+          for (int j = 0; j < n_tiles; ++j) {
+            const int kt = wk.kt0 + j, ks = steps_of(kt);
+            const uint32_t iv = base + 2 * j + 1, ik = iv + 1;
+            const bool more = j + 1 < n_tiles;
+            if (!(ok = wait_tile(iv))) break;
+            clean(iv, kt, ks);
+            if (!(ok = wait_p(0))) break;
+            pv(0, iv, ks, j == 0);
+            if (more) {
+              if (!(ok = wait_tile(ik))) break;
+              qk(0, 0, ik);
+            } else {
+              commit(o_full(0));
+            }
+            if (!(ok = wait_p(1))) break;
+            pv(1, iv, ks, j == 0);
+            commit(empty(iv % kPaSlots));
+            if (more) {
+              qk(1, 1, ik);
+              commit(empty(ik % kPaSlots));
+              if (j + 2 == n_tiles) commit(q_empty);
+            } else {
+              commit(o_full(1));
+            }
+          }
+        } else {
+          // one row tile: stream w takes tiles w, w + 2, ...; ring order K0 K1 V0 K2 V1 K3 V2 ...
+          const uint32_t base = n_tile;
+          n_tile += 2 * n_tiles;
+          auto k_at = [&](int i) { return base + (i < 2 ? (uint32_t)i : 2u * i - 1u); };
+          auto v_at = [&](int i) {      // V_i follows K_{i+1} where that exists
+            return base + (i + 1 < n_tiles ? 2u * i + 2u : 2u * i + 1u);
+          };
+          for (int i = 0; i < min(2, n_tiles); ++i) {
+            if (!(ok = wait_tile(k_at(i)))) break;
+            qk(i, 0, k_at(i));
+            commit(empty(k_at(i) % kPaSlots));
+          }
+          if (!ok) break;
+          if (n_tiles <= 2) commit(q_empty);
+          for (int i = 0; i < n_tiles; ++i) {
+            const int w = i & 1, kt = wk.kt0 + i, ks = steps_of(kt);
+            const uint32_t iv = v_at(i);
+            if (!(ok = wait_tile(iv))) break;
+            clean(iv, kt, ks);
+            if (!(ok = wait_p(w))) break;
+            pv(w, iv, ks, i < 2);
+            commit(empty(iv % kPaSlots));
+            if (i + 2 >= n_tiles) {
+              commit(o_full(w));
+            } else {
+              const uint32_t ik = k_at(i + 2);
+              if (!(ok = wait_tile(ik))) break;
+              qk(w, 0, ik);
+              commit(empty(ik % kPaSlots));
+              if (i + 3 == n_tiles) commit(q_empty);
+            }
+          }
+        }
+      }
+      // everything issued is complete, and its arrivals have landed, before the CTA goes away
+      commit(done);
+      mbar_wait_bounded(done, 0, kPollLimit);
+    } else if (warp == 10 && active) {
+      // ------------------------------------ schedule ----------------------------------- //
+      PromptItem it;
+      it.x0 = x0;
+      it.x1 = x1;
+      it.s = (int)first[0];
+      it.start(p, first[1]);
+      if (lane == 0) {
+        PromptRec r;
+        r.a = it.a; r.mid = it.x0 > it.a ? 1 : 0; r.kt0 = it.kt0; r.kt1 = it.kt1; r.n = it.n;
+        r.q0 = it.q0; r.n_tok = it.n_tok; r.h = it.h; r.pad = 0;
+        p.rec[blockIdx.x] = r;
+      }
+      uint32_t i = 0;
+      auto give = [&](const PromptWork& v) {
+        if (!pa_wait(w_empty(i), ((i / kPaWorkRing) & 1) ^ 1, abort_flag)) return false;
+        if (lane == 0) {
+          ring[i % kPaWorkRing] = v;
+          mbar_arrive(w_full(i));
+        }
+        __syncwarp();
+        ++i;
         return true;
       };
-      if (two) {
-        for (int kt = it.kt0; kt < it.kt1 && ok; ++kt) ok = load(kt, 0) && load(kt, 1);
-      } else {
-        ok = load(it.kt0, 0) && (n_tiles < 2 || load(it.kt0 + 1, 0));
-        for (int i = 0; i < n_tiles && ok; ++i)
-          ok = load(it.kt0 + i, 1) && (i + 2 >= n_tiles || load(it.kt0 + i + 2, 0));
-      }
-    } while (ok && it.next(p));
-    if (!ok) {       // give the copies in flight a bounded chance to land before the CTA goes away
-      for (uint32_t back = 1; back <= (uint32_t)kPaSlots && back <= n_tile; ++back) {
-        const uint32_t i = n_tile - back;
-        mbar_wait_bounded(full(i % kPaSlots), (i / kPaSlots) & 1, kPollLimit);
-      }
-      if (n_q) mbar_wait_bounded(q_full, (n_q - 1) & 1, kPollLimit);
+      PromptWork v;
+      bool ok = true;
+      do {
+        if (!it.mine()) continue;
+        v.n_tiles = it.kt1 - it.kt0; v.kt0 = it.kt0; v.vis = it.vis; v.len = it.seq.len;
+        v.lim0 = it.seq.len - it.seq.n + (it.q0 - it.seq.q0) + 1;
+        v.q0 = it.q0; v.n_tok = it.n_tok; v.h = it.h; v.s = it.s; v.k0 = it.seq.k0;
+        v.two = it.two(p) ? 1 : 0;
+        v.slot = it.whole() ? -1 : 2 * (int)blockIdx.x + (it.x0 > it.a ? 0 : 1);
+        ok = give(v);
+      } while (ok && it.next(p));
+      v.n_tiles = -1;
+      if (ok) give(v);
     }
-  } else if (active && warp == 9) {
-    // ------------------------------- matrix instructions ----------------------------- //
-    // The warp stays together; lane 0 issues.
-    constexpr uint32_t idesc_qk = umma_idesc(BF16, false, kPaRows, kPaKeys);
-    constexpr uint32_t idesc_pv = umma_idesc(BF16, true, kPaRows, kHeadDim);
-    uint32_t n_tile = 0, n_q = 0, n_p0 = 0, n_p1 = 0;
-    bool ok = true;
-    auto slot_of = [&](uint32_t i) { return smem + kPaRingOff + (i % kPaSlots) * kPaTileBytes; };
-    auto wait_tile = [&](uint32_t i) { return pa_wait(full(i % kPaSlots), (i / kPaSlots) & 1, abort_flag); };
-    auto qk = [&](int w, int qtile, uint32_t i) {         // S_w = Q K^T
-      if (lane == 0) {
-        const uint32_t qa = smem + qtile * kPaTileBytes, ka = slot_of(i);
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          const uint32_t off = (ks >> 2) * kPaHalfBytes + (ks & 3) * 32;
-          umma_ss(tmem + w * 128, umma_desc(qa + off, 16, 1024), umma_desc(ka + off, 16, 1024), idesc_qk, ks > 0);
-        }
-        umma_commit(s_full(w));
-      }
-      __syncwarp();
-    };
-    auto pv = [&](int w, uint32_t i, int ksteps, bool first_tile) {   // O_w (+)= P_w V
-      if (lane == 0) {
-        const uint32_t va = slot_of(i);
-        for (int ks = 0; ks < ksteps; ++ks)
-          umma_ts(tmem + kPaColO + w * 128, tmem + w * 128 + ks * 8, umma_desc(va + ks * 2048, kPaHalfBytes, 1024),
-                  idesc_pv, !first_tile || ks > 0);
-      }
-      __syncwarp();
-    };
-    // V rows of the last 16-key step that lie behind the sequence hold whatever the page holds:
-    // their weights are 0, but 0 * NaN is not, so they are cleared in shared memory.
-    auto clean = [&](uint32_t i, int kt, int ksteps) {
-      const int from = it.seq.len - kt * kPaKeys, to = ksteps * 16;
-      if (from >= to) return;
-      uint8_t* v = sgen + kPaRingOff + (i % kPaSlots) * kPaTileBytes;
-      for (int r = max(from, 0); r < to; ++r) {
-        *reinterpret_cast<uint32_t*>(v + r * 128 + lane * 4) = 0u;
-        *reinterpret_cast<uint32_t*>(v + kPaHalfBytes + r * 128 + lane * 4) = 0u;
-      }
-      fence_proxy_async();
-      __syncwarp();
-    };
-    auto steps_of = [&](int kt) { return min(8, (it.vis - kt * kPaKeys + 15) >> 4); };
-    auto wait_p = [&](int w) {
-      const bool r = w ? pa_wait(p_full(1), n_p1 & 1, abort_flag) : pa_wait(p_full(0), n_p0 & 1, abort_flag);
-      if (w) ++n_p1; else ++n_p0;
-      if (r) tc_fence_after();
-      return r;
-    };
-    auto commit = [&](uint32_t bar) { if (lane == 0) umma_commit(bar); };
-    do {
-      if (!it.mine() || it.kt1 == it.kt0) continue;
-      const bool two = it.two(p);
-      const int n_tiles = it.kt1 - it.kt0;
-      if (!(ok = pa_wait(q_full, n_q & 1, abort_flag))) break;
-      ++n_q;
-      if (two) {
-        // ring order K0 V0 K1 V1 ...: tile j's K is entry base + 2j, its V base + 2j + 1
-        const uint32_t base = n_tile;
-        n_tile += 2 * n_tiles;
-        if (!(ok = wait_tile(base))) break;
-        qk(0, 0, base);
-        qk(1, 1, base);
-        commit(empty(base % kPaSlots));
-        if (n_tiles == 1) commit(q_empty);
-        for (int j = 0; j < n_tiles; ++j) {
-          const int kt = it.kt0 + j, ks = steps_of(kt);
-          const uint32_t iv = base + 2 * j + 1, ik = iv + 1;
-          const bool more = j + 1 < n_tiles;
-          if (!(ok = wait_tile(iv))) break;
-          clean(iv, kt, ks);
-          if (!(ok = wait_p(0))) break;
-          pv(0, iv, ks, j == 0);
-          if (more) {
-            if (!(ok = wait_tile(ik))) break;
-            qk(0, 0, ik);
-          } else {
-            commit(o_full(0));
-          }
-          if (!(ok = wait_p(1))) break;
-          pv(1, iv, ks, j == 0);
-          commit(empty(iv % kPaSlots));
-          if (more) {
-            qk(1, 1, ik);
-            commit(empty(ik % kPaSlots));
-            if (j + 2 == n_tiles) commit(q_empty);
-          } else {
-            commit(o_full(1));
-          }
-        }
-      } else {
-        // one row tile: stream w takes tiles w, w + 2, ...; ring order K0 K1 V0 K2 V1 K3 V2 ...
-        const uint32_t base = n_tile;
-        n_tile += 2 * n_tiles;
-        auto k_at = [&](int i) { return base + (i < 2 ? (uint32_t)i : 2u * i - 1u); };
-        auto v_at = [&](int i) {      // V_i follows K_{i+1} where that exists
-          return base + (i + 1 < n_tiles ? 2u * i + 2u : 2u * i + 1u);
-        };
-        for (int i = 0; i < min(2, n_tiles); ++i) {
-          if (!(ok = wait_tile(k_at(i)))) break;
-          qk(i, 0, k_at(i));
-          commit(empty(k_at(i) % kPaSlots));
-        }
-        if (!ok) break;
-        if (n_tiles <= 2) commit(q_empty);
-        for (int i = 0; i < n_tiles; ++i) {
-          const int w = i & 1, kt = it.kt0 + i, ks = steps_of(kt);
-          const uint32_t iv = v_at(i);
-          if (!(ok = wait_tile(iv))) break;
-          clean(iv, kt, ks);
-          if (!(ok = wait_p(w))) break;
-          pv(w, iv, ks, i < 2);
-          commit(empty(iv % kPaSlots));
-          if (i + 2 >= n_tiles) {
-            commit(o_full(w));
-          } else {
-            const uint32_t ik = k_at(i + 2);
-            if (!(ok = wait_tile(ik))) break;
-            qk(w, 0, ik);
-            commit(empty(ik % kPaSlots));
-            if (i + 3 == n_tiles) commit(q_empty);
-          }
-        }
-      }
-    } while (ok && it.next(p));
-    // everything issued is complete, and its arrivals have landed, before the CTA goes away
-    commit(done);
-    mbar_wait_bounded(done, 0, kPollLimit);
   }
   tc_fence_before();
   __syncthreads();
