@@ -14,7 +14,7 @@
 // alternate KV tiles instead and joins their accumulators at the end.
 //
 // Warps (384 threads, one CTA per SM): 0-3 and 4-7 the two softmax warpgroups, one thread per
-// row; 8 issues the TMA loads; 9 issues the tcgen05 instructions; 10 walks the work list; 11 idle.
+// row; 8 loads Q and K, 11 loads V (TMA); 9 issues the tcgen05 instructions; 10 walks the work list.
 // TMEM: S0 S1 O0 O1, 128 columns each; the 16-bit P overwrites the first half of its S.
 // Shared memory: Q 2 x 32 KB, a ring of five 32 KB slots that K and V tiles of 128 keys take
 // turns in (K0 V0 K1 V1 ..., the order in which the products need them).
@@ -207,6 +207,18 @@ __device__ __forceinline__ bool pa_wait(uint32_t bar, uint32_t parity, volatile 
   }
 }
 
+// The same value in every lane, in a form in which the compiler knows it.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+// Place of K tile i (kv = 0) or V tile i (kv = 1) of an item with n tiles in the order in which
+// the ring is filled and read: K0 V0 K1 V1 ... for two row tiles, K0 K1 V0 K2 V1 K3 V2 ... for
+// one, whose two streams need two K tiles before the first V.
+__device__ __forceinline__ int pa_ring_pos(int two, int n, int i, int kv) {
+  if (two) return 2 * i + kv;
+  if (kv) return i + 1 < n ? 2 * i + 2 : 2 * i + 1;
+  return i < 2 ? i : 2 * i - 1;
+}
+
 __device__ __forceinline__ void store_row16(void* row, int out_dtype, int chunk, const float (&v)[8]) {
   // eight values of a row at column 8 * chunk
   if (out_dtype == 4) {
@@ -236,13 +248,13 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   auto empty = [&](int i) { return bars + 8u * (kPaSlots + i); };
   const uint32_t q_full = bars + 8u * 10, q_empty = bars + 8u * 11, done = bars + 8u * 12;
   auto s_full = [&](int w) { return bars + 8u * (13 + w); };
-  auto p_full = [&](int w) { return bars + 8u * (15 + w); };
-  auto o_full = [&](int w) { return bars + 8u * (17 + w); };
-  const uint32_t x_ready = bars + 8u * 19, x_done = bars + 8u * 20;
-  auto w_full = [&](uint32_t i) { return bars + 8u * (21 + i % kPaWorkRing); };
-  auto w_empty = [&](uint32_t i) { return bars + 8u * (21 + kPaWorkRing + i % kPaWorkRing); };
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 240);
-  uint32_t* tmem_word = reinterpret_cast<uint32_t*>(misc + 244);
+  auto o_full = [&](int w) { return bars + 8u * (15 + w); };
+  const uint32_t x_ready = bars + 8u * 17, x_done = bars + 8u * 18;
+  auto p_full = [&](int i) { return bars + 8u * (19 + i); };           // 2 * stream + half of the keys
+  auto w_full = [&](uint32_t i) { return bars + 8u * (23 + i % kPaWorkRing); };
+  auto w_empty = [&](uint32_t i) { return bars + 8u * (23 + kPaWorkRing + i % kPaWorkRing); };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 248);
+  uint32_t* tmem_word = reinterpret_cast<uint32_t*>(misc + 252);
   volatile int64_t* first = reinterpret_cast<volatile int64_t*>(misc + 256);   // s, base
   int64_t* wsum = reinterpret_cast<int64_t*>(misc + 272);                      // 12 warp sums
   PromptWork* ring = reinterpret_cast<PromptWork*>(misc + 384);                // 4 x 48 bytes
@@ -251,9 +263,10 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   if (threadIdx.x == 0) {
     for (int i = 0; i < kPaSlots; ++i) { mbar_init(full(i), 1); mbar_init(empty(i), 1); }
     mbar_init(q_full, 1); mbar_init(q_empty, 1); mbar_init(done, 1);
-    for (int w = 0; w < 2; ++w) { mbar_init(s_full(w), 1); mbar_init(p_full(w), 4); mbar_init(o_full(w), 1); }
+    for (int w = 0; w < 2; ++w) { mbar_init(s_full(w), 1); mbar_init(o_full(w), 1); }
+    for (int i = 0; i < 4; ++i) mbar_init(p_full(i), 4);
     mbar_init(x_ready, 4); mbar_init(x_done, 4);
-    for (int i = 0; i < kPaWorkRing; ++i) { mbar_init(w_full(i), 1); mbar_init(w_empty(i), 10); }
+    for (int i = 0; i < kPaWorkRing; ++i) { mbar_init(w_full(i), 1); mbar_init(w_empty(i), 11); }
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -302,7 +315,7 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   __syncthreads();
   const uint32_t tmem = *tmem_word;
 
-  // Every reader warp takes the items in turn: wait, copy, give the place back.
+  // Every reader warp (softmax 8, loads 2, matrix 1) takes the items in turn: wait, copy, give the place back.
   uint32_t n_work = 0;
   PromptWork wk;
   auto take = [&]() {
@@ -383,21 +396,22 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         for (int c = 0; c < 4; ++c) {
           uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float2 x = unpack_f32x2(fma_f32x2(pack_u32x2(sreg[c][i], sreg[c][i + 1]), sl2, ref2));
-            const float2 y = unpack_f32x2(fma_f32x2(pack_u32x2(sreg[c][i + 2], sreg[c][i + 3]), sl2, ref2));
-            const float e0 = fast_exp2(x.x), e1 = fast_exp2(x.y), e2 = fast_exp2(y.x), e3 = fast_exp2(y.y);
-            sum_a = add_f32x2(sum_a, pack_f32x2(e0, e1));
-            sum_b = add_f32x2(sum_b, pack_f32x2(e2, e3));
-            pk[i / 2] = pack2<BF16>(e0, e1);
-            pk[i / 2 + 1] = pack2<BF16>(e2, e3);
+          for (int i = 0; i < 32; i += 2) {
+            const uint64_t x2 = fma_f32x2(pack_u32x2(sreg[c][i], sreg[c][i + 1]), sl2, ref2);
+            const float2 x = unpack_f32x2(x2);
+            const uint64_t e2 = pack_f32x2(fast_exp2(x.x), fast_exp2(x.y));
+            if (i % 4) sum_b = add_f32x2(sum_b, e2); else sum_a = add_f32x2(sum_a, e2);
+            const float2 e = unpack_f32x2(e2);
+            pk[i / 2] = pack2<BF16>(e.x, e.y);
           }
           tmem_st16(ts + c * 16, pk);
+          if (c & 1) {                              // 64 keys of P are there: their product can start
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full(2 * w + (c >> 1)));
+          }
         }
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full(w));
         const float2 sa = unpack_f32x2(add_f32x2(sum_a, sum_b));
         l += sa.x + sa.y;
       }
@@ -502,71 +516,92 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     }
   } else {
     setmaxnreg_dec<kPaOtherRegs>();
-    if (warp == 8) {
-      // ------------------------------------ loads ------------------------------------ //
+    if (warp == 8 || warp == 11) {
+      // ---------------------- loads: warp 8 Q and K tiles, warp 11 V tiles --------------------- //
+      // Every operand of a TMA instruction is made uniform first: with per-lane operands (a lane
+      // per box) the instructions of a tile go out one by one at 100 cycles each, 1600 for 128
+      // keys in pages of 16, as long as the tile's products.
+      const int kv = warp == 11 ? 1 : 0;
+      const CUtensorMap* map = kv ? &vmap : &kmap;
       const int boxes = kPaKeys / p.box_tok;              // of one half tile
       const uint32_t box_bytes = (uint32_t)p.box_tok * 128u;
       const bool paged = p.seq_lens != nullptr;
-      uint32_t n_tile = 0, n_q = 0;
+      uint32_t n_tile = 0, n_q = 0, my_last = 0, my_n = 0;
       bool ok = true;
       while (ok && active && take()) {
-        const int n_tiles = wk.n_tiles;
+        const int n_tiles = uniform(wk.n_tiles), h = uniform(wk.h), two = uniform(wk.two);
         if (n_tiles == 0) continue;
         // Q: the group's heads of up to 2 * tok_tile tokens, in two halves of 64 values
-        if (!(ok = pa_wait(q_empty, (n_q & 1) ^ 1, abort_flag))) break;
-        ++n_q;
-        if (lane == 0) {
-          const uint32_t half = (uint32_t)p.tok_tile * p.group * 128u;
-          mbar_arrive_expect_tx(q_full, half * (wk.two ? 4u : 2u));
-          for (int w = 0; w < (wk.two ? 2 : 1); ++w)
-            for (int d = 0; d < 2; ++d)
-              tma_load_3d(smem + w * kPaTileBytes + d * kPaHalfBytes, &qmap, q_full, d * 64, wk.h * p.group,
-                          wk.q0 + w * p.tok_tile);
-        }
-        __syncwarp();
-        const int32_t* row = paged ? p.block_table + (int64_t)wk.s * p.bt_stride : nullptr;
-        // one tile of K (kv = 0) or V (kv = 1): lane = 2 * box + half
-        auto load = [&](int i, int kv) {
-          const int slot = n_tile % kPaSlots;
-          if (!pa_wait(empty(slot), ((n_tile / kPaSlots) & 1) ^ 1, abort_flag)) return false;
-          ++n_tile;
-          const int key0 = (wk.kt0 + i) * kPaKeys;
-          const int n_box = min(boxes, (wk.vis - key0 + p.box_tok - 1) / p.box_tok);   // >= 1
-          const uint32_t dst0 = smem + kPaRingOff + slot * kPaTileBytes;
-          const CUtensorMap* map = kv ? &vmap : &kmap;
-          if (lane == 0) mbar_arrive_expect_tx(full(slot), n_box * 2 * box_bytes);
+        if (kv == 0) {
+          if (!(ok = pa_wait(q_empty, (n_q & 1) ^ 1, abort_flag))) break;
+          ++n_q;
+          const int q0 = uniform(wk.q0);
+          if (elect_one()) {
+            const uint32_t half = (uint32_t)p.tok_tile * p.group * 128u;
+            mbar_arrive_expect_tx(q_full, half * (two ? 4u : 2u));
+            for (int w = 0; w < (two ? 2 : 1); ++w)
+              for (int d = 0; d < 2; ++d)
+                tma_load_3d(smem + w * kPaTileBytes + d * kPaHalfBytes, &qmap, q_full, d * 64, h * p.group,
+                            q0 + w * p.tok_tile);
+          }
           __syncwarp();
-          if (lane < 2 * n_box) {
-            const int b = lane >> 1, d = lane & 1;
-            const uint32_t dst = dst0 + d * kPaHalfBytes + b * box_bytes;
-            if (paged) {
-              const int key = key0 + b * p.box_tok, pg = key / p.page_size, tok = key - pg * p.page_size;
-              int page = row[pg];
-              if (page < 0 || page >= p.n_pages) {
-                if (p.status) atomicOr(p.status, kStBadPage);
-                page = 0;
+        }
+        const int kt0 = uniform(wk.kt0), vis = uniform(wk.vis), k0 = uniform(wk.k0);
+        const int32_t* row = paged ? p.block_table + (int64_t)wk.s * p.bt_stride : nullptr;
+        // lane b: the page of box b of tile i, read a few tiles ahead of its use
+        auto fetch = [&](int i) {
+          const int key = (kt0 + i) * kPaKeys + lane * p.box_tok;
+          if (!paged || i >= n_tiles || lane >= boxes || key >= vis) return 0;
+          const int page = __ldg(row + key / p.page_size);
+          if (page >= 0 && page < p.n_pages) return page;
+          if (p.status) atomicOr(p.status, kStBadPage);
+          return 0;
+        };
+        const uint32_t base = n_tile;
+        n_tile += 2 * n_tiles;
+        auto load = [&](int i, int page) {
+          const uint32_t f = base + (uint32_t)pa_ring_pos(two, n_tiles, i, kv);
+          const uint32_t slot = f % kPaSlots;
+          if (!pa_wait(empty(slot), ((f / kPaSlots) & 1) ^ 1, abort_flag)) return false;
+          my_last = f;
+          ++my_n;
+          const int key0 = (kt0 + i) * kPaKeys;
+          const int n_box = min(boxes, (vis - key0 + p.box_tok - 1) / p.box_tok);   // >= 1
+          const uint32_t dst = smem + kPaRingOff + slot * kPaTileBytes, bar = full(slot);
+          if (elect_one()) mbar_arrive_expect_tx(bar, n_box * 2 * box_bytes);
+          __syncwarp();
+          if (!paged) {
+            if (elect_one()) {
+              tma_load_4d_keep(dst, map, bar, 0, h, k0 + key0, 0);
+              tma_load_4d_keep(dst + kPaHalfBytes, map, bar, 64, h, k0 + key0, 0);
+            }
+          } else {
+            int tok = key0 % p.page_size;
+            for (int b = 0; b < n_box; ++b) {
+              const int pg = uniform(__shfl_sync(0xffffffffu, page, b));
+              const int c1 = p.head_major ? tok : h, c2 = p.head_major ? h : tok;
+              if (elect_one()) {
+                tma_load_4d_keep(dst + b * box_bytes, map, bar, 0, c1, c2, pg);
+                tma_load_4d_keep(dst + kPaHalfBytes + b * box_bytes, map, bar, 64, c1, c2, pg);
               }
-              if (p.head_major) tma_load_4d_keep(dst, map, full(slot), d * 64, tok, wk.h, page);
-              else              tma_load_4d_keep(dst, map, full(slot), d * 64, wk.h, tok, page);
-            } else {
-              tma_load_4d_keep(dst, map, full(slot), d * 64, wk.h, wk.k0 + key0, 0);
+              __syncwarp();
+              tok += p.box_tok;
+              if (tok >= p.page_size) tok = 0;
             }
           }
           __syncwarp();
           return true;
         };
-        if (wk.two) {
-          for (int i = 0; i < n_tiles && ok; ++i) ok = load(i, 0) && load(i, 1);
-        } else {
-          ok = load(0, 0) && (n_tiles < 2 || load(1, 0));
-          for (int i = 0; i < n_tiles && ok; ++i) ok = load(i, 1) && (i + 2 >= n_tiles || load(i + 2, 0));
+        int p0 = fetch(0), p1 = fetch(1), p2 = fetch(2);
+        for (int i = 0; i < n_tiles && ok; ++i) {
+          ok = load(i, p0);
+          p0 = p1;
+          p1 = p2;
+          p2 = fetch(i + 3);
         }
       }
       if (*abort_flag) {   // give the copies in flight a bounded chance to land before the CTA goes away
-        for (uint32_t back = 1; back <= (uint32_t)kPaSlots && back <= n_tile; ++back) {
-          const uint32_t i = n_tile - back;
-          mbar_wait_bounded(full(i % kPaSlots), (i / kPaSlots) & 1, kPollLimit);
-        }
+        if (my_n) mbar_wait_bounded(full(my_last % kPaSlots), (my_last / kPaSlots) & 1, kPollLimit);
         if (n_q) mbar_wait_bounded(q_full, (n_q - 1) & 1, kPollLimit);
       }
     } else if (warp == 9) {
@@ -593,19 +628,27 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         }
         __syncwarp();
       };
-      auto pv = [&](int w, uint32_t i, int ksteps, bool first_tile) {   // O_w (+)= P_w V
+      // O_w (+)= P_w V, in two halves of the keys as P arrives
+      auto pv = [&](int w, uint32_t i, int ksteps, bool first_tile) {
         const uint32_t va = ring_v + (i % kPaSlots) * tile16, keep = first_tile ? 0u : 1u;
-        if (elect_one()) {
-          if (ksteps == 8) {
+        const uint32_t phase = w ? n_p1++ : n_p0++;
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks)
-              umma_ts(tm + kPaColO + w * 128, tm + w * 128 + ks * 8, va + ks * 128, hi, idesc_pv, ks > 0 ? 1u : keep);
-          } else {
-            for (int ks = 0; ks < ksteps; ++ks)
-              umma_ts(tm + kPaColO + w * 128, tm + w * 128 + ks * 8, va + ks * 128, hi, idesc_pv, ks > 0 ? 1u : keep);
+        for (int half = 0; half < 2; ++half) {
+          if (!pa_wait(p_full(2 * w + half), phase & 1, abort_flag)) return false;
+          tc_fence_after();
+          if (elect_one()) {
+            if (ksteps == 8) {
+#pragma unroll
+              for (int ks = 4 * half; ks < 4 * half + 4; ++ks)
+                umma_ts(tm + kPaColO + w * 128, tm + w * 128 + ks * 8, va + ks * 128, hi, idesc_pv, ks > 0 ? 1u : keep);
+            } else {
+              for (int ks = 4 * half; ks < min(4 * half + 4, ksteps); ++ks)
+                umma_ts(tm + kPaColO + w * 128, tm + w * 128 + ks * 8, va + ks * 128, hi, idesc_pv, ks > 0 ? 1u : keep);
+            }
           }
+          __syncwarp();
         }
-        __syncwarp();
+        return true;
       };
       // V rows of the last 16-key step that lie behind the sequence hold whatever the page holds:
       // their weights are 0, but 0 * NaN is not, so they are cleared in shared memory.
@@ -621,16 +664,10 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         __syncwarp();
       };
       auto steps_of = [&](int kt) { return min(8, (wk.vis - kt * kPaKeys + 15) >> 4); };
-      auto wait_p = [&](int w) {
-        const bool r = w ? pa_wait(p_full(1), n_p1 & 1, abort_flag) : pa_wait(p_full(0), n_p0 & 1, abort_flag);
-        if (w) ++n_p1; else ++n_p0;
-        if (r) tc_fence_after();
-        return r;
-      };
       // (all commits from one thread: elect_one picks the same lane every time)
       auto commit = [&](uint32_t bar) { if (elect_one()) umma_commit(bar); __syncwarp(); };
       while (ok && active && take()) {
-        const int n_tiles = __shfl_sync(0xffffffffu, wk.n_tiles, 0);     // uniform, and known to be
+        const int n_tiles = uniform(wk.n_tiles);
         if (n_tiles == 0) continue;
         if (!(ok = pa_wait(q_full, n_q & 1, abort_flag))) break;
         ++n_q;
@@ -649,16 +686,14 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
             const bool more = j + 1 < n_tiles;
             if (!(ok = wait_tile(iv))) break;
             clean(iv, kt, ks);
-            if (!(ok = wait_p(0))) break;
-            pv(0, iv, ks, j == 0);
+            if (!(ok = pv(0, iv, ks, j == 0))) break;
             if (more) {
               if (!(ok = wait_tile(ik))) break;
               qk(0, 0, ik);
             } else {
               commit(o_full(0));
             }
-            if (!(ok = wait_p(1))) break;
-            pv(1, iv, ks, j == 0);
+            if (!(ok = pv(1, iv, ks, j == 0))) break;
             commit(empty(iv % kPaSlots));
             if (more) {
               qk(1, 1, ik);
@@ -672,10 +707,8 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           // one row tile: stream w takes tiles w, w + 2, ...; ring order K0 K1 V0 K2 V1 K3 V2 ...
           const uint32_t base = n_tile;
           n_tile += 2 * n_tiles;
-          auto k_at = [&](int i) { return base + (i < 2 ? (uint32_t)i : 2u * i - 1u); };
-          auto v_at = [&](int i) {      // V_i follows K_{i+1} where that exists
-            return base + (i + 1 < n_tiles ? 2u * i + 2u : 2u * i + 1u);
-          };
+          auto k_at = [&](int i) { return base + (uint32_t)pa_ring_pos(0, n_tiles, i, 0); };
+          auto v_at = [&](int i) { return base + (uint32_t)pa_ring_pos(0, n_tiles, i, 1); };
           for (int i = 0; i < min(2, n_tiles); ++i) {
             if (!(ok = wait_tile(k_at(i)))) break;
             qk(i, 0, k_at(i));
@@ -688,8 +721,7 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
             const uint32_t iv = v_at(i);
             if (!(ok = wait_tile(iv))) break;
             clean(iv, kt, ks);
-            if (!(ok = wait_p(w))) break;
-            pv(w, iv, ks, i < 2);
+            if (!(ok = pv(w, iv, ks, i < 2))) break;
             commit(empty(iv % kPaSlots));
             if (i + 2 >= n_tiles) {
               commit(o_full(w));
