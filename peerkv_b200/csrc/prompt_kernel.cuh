@@ -14,10 +14,10 @@
 // alternate KV tiles instead and joins their accumulators at the end.
 //
 // Warps (384 threads, one CTA per SM): 0-3 and 4-7 the two softmax warpgroups, one thread per
-// row; 8 loads Q and K, 11 loads V (TMA); 9 issues the tcgen05 instructions; 10 walks the work list.
+// row; 8 walks the work list and loads Q and K, 11 loads V (TMA); 9 and 10 issue the tcgen05
+// instructions of the two row tiles.
 // TMEM: S0 S1 O0 O1, 128 columns each; the 16-bit P overwrites the first half of its S.
-// Shared memory: Q 2 x 32 KB, a ring of five 32 KB slots that K and V tiles of 128 keys take
-// turns in (K0 V0 K1 V1 ..., the order in which the products need them).
+// Shared memory: Q 2 x 32 KB; K and V tiles of 128 keys in rings of two and three 32 KB slots.
 //
 // Sums.  Scores, maxima, sums and O are fp32.  P is rounded to the 16-bit type of V, as the
 // matrix instruction wants both operands alike; the row sum adds the unrounded values.  The
@@ -39,7 +39,7 @@ namespace pkv {
 constexpr int kPaRows = 128;       // rows of a row tile (TMEM lanes)
 constexpr int kPaKeys = 128;       // keys of a KV tile
 constexpr int kPaThreads = 384;
-constexpr int kPaSlots = 5;
+constexpr int kPaKSlots = 2, kPaVSlots = 3, kPaSlots = kPaKSlots + kPaVSlots;
 constexpr int kPaTileBytes = kPaKeys * kHeadDim * 2;     // 32 KB
 constexpr int kPaHalfBytes = kPaTileBytes / 2;           // 128 rows x 64 values, 128-byte swizzle
 constexpr int kPaRingOff = 2 * kPaTileBytes;
@@ -210,14 +210,11 @@ __device__ __forceinline__ bool pa_wait(uint32_t bar, uint32_t parity, volatile 
 // The same value in every lane, in a form in which the compiler knows it.
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
-// Place of K tile i (kv = 0) or V tile i (kv = 1) of an item with n tiles in the order in which
-// the ring is filled and read: K0 V0 K1 V1 ... for two row tiles, K0 K1 V0 K2 V1 K3 V2 ... for
-// one, whose two streams need two K tiles before the first V.
-__device__ __forceinline__ int pa_ring_pos(int two, int n, int i, int kv) {
-  if (two) return 2 * i + kv;
-  if (kv) return i + 1 < n ? 2 * i + 2 : 2 * i + 1;
-  return i < 2 ? i : 2 * i - 1;
-}
+// The K tiles have a ring of two slots, the V tiles one of three: slot and phase parity of the
+// i-th tile a CTA loads.  (Two rings, each filled by one warp, which has waited for a slot's
+// last release before it fills it: so no wait can mistake one round of a slot for another.)
+__device__ __forceinline__ uint32_t pa_slot(int kv, uint32_t i) { return kv ? kPaKSlots + i % kPaVSlots : i % kPaKSlots; }
+__device__ __forceinline__ uint32_t pa_phase(int kv, uint32_t i) { return (kv ? i / kPaVSlots : i / kPaKSlots) & 1; }
 
 __device__ __forceinline__ void store_row16(void* row, int out_dtype, int chunk, const float (&v)[8]) {
   // eight values of a row at column 8 * chunk
@@ -251,19 +248,20 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   auto o_full = [&](int w) { return bars + 8u * (15 + w); };
   const uint32_t x_ready = bars + 8u * 17, x_done = bars + 8u * 18;
   auto p_full = [&](int i) { return bars + 8u * (19 + i); };           // 2 * stream + half of the keys
-  auto w_full = [&](uint32_t i) { return bars + 8u * (23 + i % kPaWorkRing); };
-  auto w_empty = [&](uint32_t i) { return bars + 8u * (23 + kPaWorkRing + i % kPaWorkRing); };
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 248);
-  uint32_t* tmem_word = reinterpret_cast<uint32_t*>(misc + 252);
-  volatile int64_t* first = reinterpret_cast<volatile int64_t*>(misc + 256);   // s, base
-  int64_t* wsum = reinterpret_cast<int64_t*>(misc + 272);                      // 12 warp sums
-  PromptWork* ring = reinterpret_cast<PromptWork*>(misc + 384);                // 4 x 48 bytes
+  auto turn = [&](int w) { return bars + 8u * (23 + w); };
+  auto w_full = [&](uint32_t i) { return bars + 8u * (25 + i % kPaWorkRing); };
+  auto w_empty = [&](uint32_t i) { return bars + 8u * (25 + kPaWorkRing + i % kPaWorkRing); };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 272);
+  uint32_t* tmem_word = reinterpret_cast<uint32_t*>(misc + 276);
+  volatile int64_t* first = reinterpret_cast<volatile int64_t*>(misc + 280);   // s, base
+  int64_t* wsum = reinterpret_cast<int64_t*>(misc + 296);                      // 12 warp sums
+  PromptWork* ring = reinterpret_cast<PromptWork*>(misc + 400);                // 4 x 48 bytes
   float2* xml = reinterpret_cast<float2*>(misc + 640);                         // [128] (m, l) of stream 1
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kPaSlots; ++i) { mbar_init(full(i), 1); mbar_init(empty(i), 1); }
-    mbar_init(q_full, 1); mbar_init(q_empty, 1); mbar_init(done, 1);
-    for (int w = 0; w < 2; ++w) { mbar_init(s_full(w), 1); mbar_init(o_full(w), 1); }
+    for (int i = 0; i < kPaSlots; ++i) { mbar_init(full(i), 1); mbar_init(empty(i), 2); }
+    mbar_init(q_full, 1); mbar_init(q_empty, 2); mbar_init(done, 2);
+    for (int w = 0; w < 2; ++w) { mbar_init(s_full(w), 1); mbar_init(o_full(w), 1); mbar_init(turn(w), 1); }
     for (int i = 0; i < 4; ++i) mbar_init(p_full(i), 4);
     mbar_init(x_ready, 4); mbar_init(x_done, 4);
     for (int i = 0; i < kPaWorkRing; ++i) { mbar_init(w_full(i), 1); mbar_init(w_empty(i), 11); }
@@ -315,7 +313,7 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   __syncthreads();
   const uint32_t tmem = *tmem_word;
 
-  // Every reader warp (softmax 8, loads 2, matrix 1) takes the items in turn: wait, copy, give the place back.
+  // Every reader warp (softmax 8, matrix 2, V loads 1) takes the items in turn: wait, copy, give the place back.
   uint32_t n_work = 0;
   PromptWork wk;
   auto take = [&]() {
@@ -360,58 +358,79 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
             for (int i = 0; i < 32; ++i)
               if (c * 32 + i >= left) sreg[c][i] = 0xff800000u;           // -inf
         }
-        float mx[4];
+        auto row_max = [&]() {
+          float mx[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          mx[c] = fmaxf(__uint_as_float(sreg[c][0]), __uint_as_float(sreg[c][1]));
+          for (int c = 0; c < 4; ++c) {
+            mx[c] = fmaxf(__uint_as_float(sreg[c][0]), __uint_as_float(sreg[c][1]));
 #pragma unroll
-          for (int i = 2; i < 32; i += 2)
-            mx[c] = max3(mx[c], __uint_as_float(sreg[c][i]), __uint_as_float(sreg[c][i + 1]));
-        }
-        const float tile_max = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        if (j == 0) {
-          m = tile_max;
-        } else if (__any_sync(0xffffffffu, (tile_max - m) * sl > 8.f)) {
+            for (int i = 2; i < 32; i += 2)
+              mx[c] = max3(mx[c], __uint_as_float(sreg[c][i]), __uint_as_float(sreg[c][i + 1]));
+          }
+          return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        };
+        const uint64_t sl2 = pack_f32x2(sl, sl);
+        uint64_t ref2, sum_a, sum_b;                                       // two fp32 sums each
+        // a row that has seen no key yet has m = -inf: 0 as the reference keeps exp2(-inf) = 0
+        auto set_ref = [&]() { const float ref = m == -INFINITY ? 0.f : -m * sl; ref2 = pack_f32x2(ref, ref); };
+        float mx0 = -INFINITY, mx1 = -INFINITY;
+        auto exps = [&](int half, bool with_max) {                         // 64 keys: P and its sums
+          if (half == 0) sum_a = sum_b = 0;
+#pragma unroll
+          for (int c = 2 * half; c < 2 * half + 2; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const uint64_t x2 = fma_f32x2(pack_u32x2(sreg[c][i], sreg[c][i + 1]), sl2, ref2);
+              const float2 x = unpack_f32x2(x2);
+              const uint64_t e2 = pack_f32x2(fast_exp2(x.x), fast_exp2(x.y));
+              if (with_max) {      // of this half and of the other one, where the exponentials leave room
+                mx0 = max3(mx0, __uint_as_float(sreg[c][i]), __uint_as_float(sreg[c][i + 1]));
+                mx1 = max3(mx1, __uint_as_float(sreg[c ^ 2][i]), __uint_as_float(sreg[c ^ 2][i + 1]));
+              }
+              if (i % 4) sum_b = add_f32x2(sum_b, e2); else sum_a = add_f32x2(sum_a, e2);
+              const float2 e = unpack_f32x2(e2);
+              pk[i / 2] = pack2<BF16>(e.x, e.y);
+            }
+            tmem_st16(ts + c * 16, pk);
+          }
+        };
+        auto hand_over = [&](int half) {                                   // its product can start
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_full(2 * w + half));
+        };
+        // The exponentials start with the reference of the tiles before, beside the search for this
+        // tile's maximum; only if that lies more than 2^8 above are they done again.
+        if (j == 0) m = row_max();
+        set_ref();
+        exps(0, true);
+        const float tile_max = fmaxf(mx0, mx1);
+        if (__any_sync(0xffffffffu, (tile_max - m) * sl > 8.f)) {
           // The product that wrote O last is complete: the scores just waited for were issued
           // behind it, and the next one waits for this warpgroup.
           const float mn = fmaxf(m, tile_max);
           const float alpha = m == -INFINITY ? 0.f : fast_exp2((m - mn) * sl);
           l *= alpha;
           m = mn;
+          set_ref();
+          if (j > 0) {
 #pragma unroll 1
-          for (int c = 0; c < 8; ++c) {
-            uint32_t o[16];
-            tmem_ld16(o, to + c * 16);
-            tmem_wait_ld();
+            for (int c = 0; c < 8; ++c) {
+              uint32_t o[16];
+              tmem_ld16(o, to + c * 16);
+              tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            tmem_st16(to + c * 16, o);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st16(to + c * 16, o);
+            }
           }
+          exps(0, false);
         }
-        // a row that has seen no key yet has m = -inf: 0 as the reference keeps exp2(-inf) = 0
-        const float ref = m == -INFINITY ? 0.f : -m * sl;
-        const uint64_t sl2 = pack_f32x2(sl, sl), ref2 = pack_f32x2(ref, ref);
-        uint64_t sum_a = 0, sum_b = 0;                                     // two fp32 sums each
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const uint64_t x2 = fma_f32x2(pack_u32x2(sreg[c][i], sreg[c][i + 1]), sl2, ref2);
-            const float2 x = unpack_f32x2(x2);
-            const uint64_t e2 = pack_f32x2(fast_exp2(x.x), fast_exp2(x.y));
-            if (i % 4) sum_b = add_f32x2(sum_b, e2); else sum_a = add_f32x2(sum_a, e2);
-            const float2 e = unpack_f32x2(e2);
-            pk[i / 2] = pack2<BF16>(e.x, e.y);
-          }
-          tmem_st16(ts + c * 16, pk);
-          if (c & 1) {                              // 64 keys of P are there: their product can start
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_full(2 * w + (c >> 1)));
-          }
-        }
+        hand_over(0);
+        exps(1, false);
+        hand_over(1);
         const float2 sa = unpack_f32x2(add_f32x2(sum_a, sum_b));
         l += sa.x + sa.y;
       }
@@ -517,7 +536,7 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   } else {
     setmaxnreg_dec<kPaOtherRegs>();
     if (warp == 8 || warp == 11) {
-      // ---------------------- loads: warp 8 Q and K tiles, warp 11 V tiles --------------------- //
+      // ------------ work list, Q and K tiles: warp 8; V tiles: warp 11 ------------ //
       // Every operand of a TMA instruction is made uniform first: with per-lane operands (a lane
       // per box) the instructions of a tile go out one by one at 100 cycles each, 1600 for 128
       // keys in pages of 16, as long as the tile's products.
@@ -526,9 +545,47 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       const int boxes = kPaKeys / p.box_tok;              // of one half tile
       const uint32_t box_bytes = (uint32_t)p.box_tok * 128u;
       const bool paged = p.seq_lens != nullptr;
-      uint32_t n_tile = 0, n_q = 0, my_last = 0, my_n = 0;
-      bool ok = true;
-      while (ok && active && take()) {
+      uint32_t n_tile = 0, n_q = 0;                       // tiles and Q loads issued
+      bool ok = active;
+      PromptItem it;
+      uint32_t n_given = 0;
+      // the work list: what this warp puts into the ring the other warps take out
+      auto give = [&](const PromptWork& v) {
+        if (!pa_wait(w_empty(n_given), ((n_given / kPaWorkRing) & 1) ^ 1, abort_flag)) return false;
+        if (lane == 0) {
+          ring[n_given % kPaWorkRing] = v;
+          mbar_arrive(w_full(n_given));
+        }
+        __syncwarp();
+        ++n_given;
+        return v.n_tiles >= 0;
+      };
+      auto make = [&]() {
+        bool have = true;
+        if (n_given == 0) {
+          it.x0 = x0;
+          it.x1 = x1;
+          it.s = (int)first[0];
+          it.start(p, first[1]);
+          if (lane == 0) {
+            PromptRec r;
+            r.a = it.a; r.mid = it.x0 > it.a ? 1 : 0; r.kt0 = it.kt0; r.kt1 = it.kt1; r.n = it.n;
+            r.q0 = it.q0; r.n_tok = it.n_tok; r.h = it.h; r.pad = 0;
+            p.rec[blockIdx.x] = r;
+          }
+        } else {
+          have = it.next(p);
+        }
+        while (have && !it.mine()) have = it.next(p);
+        wk.n_tiles = have ? it.kt1 - it.kt0 : -1;
+        wk.kt0 = it.kt0; wk.vis = it.vis; wk.len = it.seq.len;
+        wk.lim0 = it.seq.len - it.seq.n + (it.q0 - it.seq.q0) + 1;
+        wk.q0 = it.q0; wk.n_tok = it.n_tok; wk.h = it.h; wk.s = it.s; wk.k0 = it.seq.k0;
+        wk.two = it.two(p) ? 1 : 0;
+        wk.slot = it.whole() ? -1 : 2 * (int)blockIdx.x + (it.x0 > it.a ? 0 : 1);
+        return give(wk);
+      };
+      while (ok && (kv == 0 ? make() : take())) {
         const int n_tiles = uniform(wk.n_tiles), h = uniform(wk.h), two = uniform(wk.two);
         if (n_tiles == 0) continue;
         // Q: the group's heads of up to 2 * tok_tile tokens, in two halves of 64 values
@@ -557,14 +614,10 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           if (p.status) atomicOr(p.status, kStBadPage);
           return 0;
         };
-        const uint32_t base = n_tile;
-        n_tile += 2 * n_tiles;
         auto load = [&](int i, int page) {
-          const uint32_t f = base + (uint32_t)pa_ring_pos(two, n_tiles, i, kv);
-          const uint32_t slot = f % kPaSlots;
-          if (!pa_wait(empty(slot), ((f / kPaSlots) & 1) ^ 1, abort_flag)) return false;
-          my_last = f;
-          ++my_n;
+          const uint32_t slot = pa_slot(kv, n_tile);
+          if (!pa_wait(empty(slot), pa_phase(kv, n_tile) ^ 1, abort_flag)) return false;
+          ++n_tile;
           const int key0 = (kt0 + i) * kPaKeys;
           const int n_box = min(boxes, (vis - key0 + p.box_tok - 1) / p.box_tok);   // >= 1
           const uint32_t dst = smem + kPaRingOff + slot * kPaTileBytes, bar = full(slot);
@@ -601,23 +654,27 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         }
       }
       if (*abort_flag) {   // give the copies in flight a bounded chance to land before the CTA goes away
-        if (my_n) mbar_wait_bounded(full(my_last % kPaSlots), (my_last / kPaSlots) & 1, kPollLimit);
+        for (uint32_t back = 1; back <= (uint32_t)(kv ? kPaVSlots : kPaKSlots) && back <= n_tile; ++back)
+          mbar_wait_bounded(full(pa_slot(kv, n_tile - back)), pa_phase(kv, n_tile - back), kPollLimit);
         if (n_q) mbar_wait_bounded(q_full, (n_q - 1) & 1, kPollLimit);
       }
-    } else if (warp == 9) {
+    } else {
       // ------------------------------- matrix instructions ----------------------------- //
-      // The warp stays together; one elected lane issues.
+      // Warp 9 issues stream 0's, warp 10 stream 1's: one warp for both spent as long on waits and
+      // issue between the products as the products took.  The warp stays together; one elected
+      // lane issues.  Every ring slot is given back by both streams.
       constexpr uint32_t idesc_qk = umma_idesc(BF16, false, kPaRows, kPaKeys);
       constexpr uint32_t idesc_pv = umma_idesc(BF16, true, kPaRows, kHeadDim);
-      uint32_t n_tile = 0, n_q = 0, n_p0 = 0, n_p1 = 0;
+      const int w = warp - 9;
+      uint32_t n_tile = 0, n_q = 0, n_p = 0, n_turn = 0;
       bool ok = true;
-      auto wait_tile = [&](uint32_t i) { return pa_wait(full(i % kPaSlots), (i / kPaSlots) & 1, abort_flag); };
+      auto wait_tile = [&](int kv, uint32_t i) { return pa_wait(full(pa_slot(kv, i)), pa_phase(kv, i), abort_flag); };
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t q_lo = umma_desc_lo(smem, 16), ring_k = umma_desc_lo(smem + kPaRingOff, 16),
                      ring_v = umma_desc_lo(smem + kPaRingOff, kPaHalfBytes);
       constexpr uint32_t hi = umma_desc_hi(1024), tile16 = kPaTileBytes / 16, half16 = kPaHalfBytes / 16;
-      auto qk = [&](int w, int qtile, uint32_t i) {         // S_w = Q K^T
-        const uint32_t qa = q_lo + qtile * tile16, ka = ring_k + (i % kPaSlots) * tile16;
+      auto qk = [&](int qtile, uint32_t i) {         // S_w = Q K^T
+        const uint32_t qa = q_lo + qtile * tile16, ka = ring_k + pa_slot(0, i) * tile16;
         if (elect_one()) {
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks) {
@@ -629,12 +686,13 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         __syncwarp();
       };
       // O_w (+)= P_w V, in two halves of the keys as P arrives
-      auto pv = [&](int w, uint32_t i, int ksteps, bool first_tile) {
-        const uint32_t va = ring_v + (i % kPaSlots) * tile16, keep = first_tile ? 0u : 1u;
-        const uint32_t phase = w ? n_p1++ : n_p0++;
+      auto pv = [&](uint32_t i, int ksteps, bool first_tile, bool in_turn) {
+        const uint32_t va = ring_v + pa_slot(1, i) * tile16, keep = first_tile ? 0u : 1u;
+        const uint32_t phase = n_p++;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           if (!pa_wait(p_full(2 * w + half), phase & 1, abort_flag)) return false;
+          if (in_turn && half == 0 && !pa_wait(turn(w), (n_turn++ & 1) ^ (w == 0 ? 1u : 0u), abort_flag)) return false;
           tc_fence_after();
           if (elect_one()) {
             if (ksteps == 8) {
@@ -654,8 +712,7 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       // their weights are 0, but 0 * NaN is not, so they are cleared in shared memory.
       auto clean = [&](uint32_t i, int kt, int ksteps) {
         const int from = wk.len - kt * kPaKeys, to = ksteps * 16;
-        if (from >= to) return;
-        uint8_t* v = sgen + kPaRingOff + (i % kPaSlots) * kPaTileBytes;
+        uint8_t* v = sgen + kPaRingOff + pa_slot(1, i) * kPaTileBytes;
         for (int r = max(from, 0); r < to; ++r) {
           *reinterpret_cast<uint32_t*>(v + r * 128 + lane * 4) = 0u;
           *reinterpret_cast<uint32_t*>(v + kPaHalfBytes + r * 128 + lane * 4) = 0u;
@@ -663,74 +720,69 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         fence_proxy_async();
         __syncwarp();
       };
-      auto steps_of = [&](int kt) { return min(8, (wk.vis - kt * kPaKeys + 15) >> 4); };
       // (all commits from one thread: elect_one picks the same lane every time)
       auto commit = [&](uint32_t bar) { if (elect_one()) umma_commit(bar); __syncwarp(); };
+      auto give_back = [&](int kv, uint32_t i) { commit(empty(pa_slot(kv, i))); };
       while (ok && active && take()) {
         const int n_tiles = uniform(wk.n_tiles);
         if (n_tiles == 0) continue;
         if (!(ok = pa_wait(q_full, n_q & 1, abort_flag))) break;
         ++n_q;
-        if (wk.two) {
-          // ring order K0 V0 K1 V1 ...: tile j's K is entry base + 2j, its V base + 2j + 1
-          const uint32_t base = n_tile;
-          n_tile += 2 * n_tiles;
-          if (!(ok = wait_tile(base))) break;
-          qk(0, 0, base);
-          qk(1, 1, base);
-          commit(empty(base % kPaSlots));
+        const uint32_t base = n_tile;
+        n_tile += n_tiles;
+        // V tile i of the item: product and release
+        auto values = [&](int i, bool first_tile, bool in_turn) {
+          const int kt = wk.kt0 + i, ks = min(8, (wk.vis - kt * kPaKeys + 15) >> 4);
+          if (!wait_tile(1, base + i)) return false;
+          if (ks * 16 > wk.len - kt * kPaKeys) clean(base + i, kt, ks);
+          if (!pv(base + i, ks, first_tile, in_turn)) return false;
+          give_back(1, base + i);
+          return true;
+        };
+        auto scores = [&](int i, int qtile) {
+          if (!wait_tile(0, base + i)) return false;
+          qk(qtile, base + i);
+          give_back(0, base + i);
+          return true;
+        };
+        if (uniform(wk.two)) {
+          // Both streams take every tile, and they issue in turn: O_0 (+)= P_0 V and the next S_0, then
+          // the same of stream 1.  Left alone they fall into step, and the exponentials of both
+          // wait for the tensor cores and then compete (measured: 4300 cycles a step instead of
+          // 3100).
+          auto pass_turn = [&]() { if (elect_one()) mbar_arrive(turn(w ^ 1)); __syncwarp(); };
+          ok = scores(0, w);
           if (n_tiles == 1) commit(q_empty);
-          for (int j = 0; j < n_tiles; ++j) {
-            const int kt = wk.kt0 + j, ks = steps_of(kt);
-            const uint32_t iv = base + 2 * j + 1, ik = iv + 1;
-            const bool more = j + 1 < n_tiles;
-            if (!(ok = wait_tile(iv))) break;
-            clean(iv, kt, ks);
-            if (!(ok = pv(0, iv, ks, j == 0))) break;
-            if (more) {
-              if (!(ok = wait_tile(ik))) break;
-              qk(0, 0, ik);
-            } else {
-              commit(o_full(0));
-            }
-            if (!(ok = pv(1, iv, ks, j == 0))) break;
-            commit(empty(iv % kPaSlots));
-            if (more) {
-              qk(1, 1, ik);
-              commit(empty(ik % kPaSlots));
-              if (j + 2 == n_tiles) commit(q_empty);
-            } else {
-              commit(o_full(1));
-            }
-          }
-        } else {
-          // one row tile: stream w takes tiles w, w + 2, ...; ring order K0 K1 V0 K2 V1 K3 V2 ...
-          const uint32_t base = n_tile;
-          n_tile += 2 * n_tiles;
-          auto k_at = [&](int i) { return base + (uint32_t)pa_ring_pos(0, n_tiles, i, 0); };
-          auto v_at = [&](int i) { return base + (uint32_t)pa_ring_pos(0, n_tiles, i, 1); };
-          for (int i = 0; i < min(2, n_tiles); ++i) {
-            if (!(ok = wait_tile(k_at(i)))) break;
-            qk(i, 0, k_at(i));
-            commit(empty(k_at(i) % kPaSlots));
-          }
-          if (!ok) break;
-          if (n_tiles <= 2) commit(q_empty);
-          for (int i = 0; i < n_tiles; ++i) {
-            const int w = i & 1, kt = wk.kt0 + i, ks = steps_of(kt);
-            const uint32_t iv = v_at(i);
-            if (!(ok = wait_tile(iv))) break;
-            clean(iv, kt, ks);
-            if (!(ok = pv(w, iv, ks, i < 2))) break;
-            commit(empty(iv % kPaSlots));
-            if (i + 2 >= n_tiles) {
+          for (int j = 0; j < n_tiles && ok; ++j) {
+            if (!(ok = values(j, j == 0, true))) break;
+            if (j + 1 == n_tiles) {
               commit(o_full(w));
             } else {
-              const uint32_t ik = k_at(i + 2);
-              if (!(ok = wait_tile(ik))) break;
-              qk(w, 0, ik);
-              commit(empty(ik % kPaSlots));
+              ok = scores(j + 1, w);
+              if (j + 2 == n_tiles) commit(q_empty);
+            }
+            pass_turn();
+          }
+        } else {
+          // one row tile: stream w takes tiles w, w + 2, ..., and lets the others pass, so that no
+          // slot is filled again before both have seen it
+          auto pass = [&](int kv, int i) {
+            if (!wait_tile(kv, base + i)) return false;
+            if (elect_one()) mbar_arrive(empty(pa_slot(kv, base + i)));
+            __syncwarp();
+            return true;
+          };
+          ok = w == 0 ? scores(0, 0) : pass(0, 0);
+          if (ok && n_tiles > 1) ok = w == 1 ? scores(1, 0) : pass(0, 1);
+          if (n_tiles <= 2) commit(q_empty);
+          for (int i = 0; i < n_tiles && ok; ++i) {
+            const bool mine = (i & 1) == w;
+            if (!(ok = mine ? values(i, i < 2, false) : pass(1, i))) break;
+            if (i + 2 < n_tiles) {
+              ok = mine ? scores(i + 2, 0) : pass(0, i + 2);
               if (i + 3 == n_tiles) commit(q_empty);
+            } else if (mine) {
+              commit(o_full(w));
             }
           }
         }
@@ -738,43 +790,6 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       // everything issued is complete, and its arrivals have landed, before the CTA goes away
       commit(done);
       mbar_wait_bounded(done, 0, kPollLimit);
-    } else if (warp == 10 && active) {
-      // ------------------------------------ schedule ----------------------------------- //
-      PromptItem it;
-      it.x0 = x0;
-      it.x1 = x1;
-      it.s = (int)first[0];
-      it.start(p, first[1]);
-      if (lane == 0) {
-        PromptRec r;
-        r.a = it.a; r.mid = it.x0 > it.a ? 1 : 0; r.kt0 = it.kt0; r.kt1 = it.kt1; r.n = it.n;
-        r.q0 = it.q0; r.n_tok = it.n_tok; r.h = it.h; r.pad = 0;
-        p.rec[blockIdx.x] = r;
-      }
-      uint32_t i = 0;
-      auto give = [&](const PromptWork& v) {
-        if (!pa_wait(w_empty(i), ((i / kPaWorkRing) & 1) ^ 1, abort_flag)) return false;
-        if (lane == 0) {
-          ring[i % kPaWorkRing] = v;
-          mbar_arrive(w_full(i));
-        }
-        __syncwarp();
-        ++i;
-        return true;
-      };
-      PromptWork v;
-      bool ok = true;
-      do {
-        if (!it.mine()) continue;
-        v.n_tiles = it.kt1 - it.kt0; v.kt0 = it.kt0; v.vis = it.vis; v.len = it.seq.len;
-        v.lim0 = it.seq.len - it.seq.n + (it.q0 - it.seq.q0) + 1;
-        v.q0 = it.q0; v.n_tok = it.n_tok; v.h = it.h; v.s = it.s; v.k0 = it.seq.k0;
-        v.two = it.two(p) ? 1 : 0;
-        v.slot = it.whole() ? -1 : 2 * (int)blockIdx.x + (it.x0 > it.a ? 0 : 1);
-        ok = give(v);
-      } while (ok && it.next(p));
-      v.n_tiles = -1;
-      if (ok) give(v);
     }
   }
   tc_fence_before();

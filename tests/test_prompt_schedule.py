@@ -1,7 +1,7 @@
 """The work split of the prompt-attention kernel, restated on the host: every KV tile of every
 item is done exactly once, a CTA's pieces never share a workspace slot, the join finds exactly
-the pieces that were written, and the ring of K / V tiles is filled in the order in which the
-matrix-instruction warp reads it."""
+the pieces that were written, and the two streams of products never wait for a tile that waits
+for them."""
 import os
 import random
 import re
@@ -13,11 +13,11 @@ SRC = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__
 
 
 def const(name):
-    return int(re.search(r"constexpr int %s = (\d+)" % name, SRC).group(1))
+    return int(re.search(r"constexpr int [^;]*?\b%s = (\d+)" % name, SRC).group(1))
 
 
-ITEM_COST, MIN_PIECE, KEYS, ROWS, SLOTS = (const(n) for n in ("kPaItemCost", "kPaMinPiece", "kPaKeys", "kPaRows",
-                                                              "kPaSlots"))
+ITEM_COST, MIN_PIECE, KEYS, ROWS, K_SLOTS, V_SLOTS = (
+    const(n) for n in ("kPaItemCost", "kPaMinPiece", "kPaKeys", "kPaRows", "kPaKSlots", "kPaVSlots"))
 
 
 def items(seqs, hkv, group, causal):
@@ -124,35 +124,54 @@ def test_edge_lengths():
             check([(n, length)], 8, 4, causal, 148)
 
 
-def ring_order(n_tiles, two):
-    """Order in which the load warp fills the ring."""
-    if two:
-        return [x for j in range(n_tiles) for x in (("K", j), ("V", j))]
-    out = [("K", 0)] + ([("K", 1)] if n_tiles > 1 else [])
-    for i in range(n_tiles):
-        out.append(("V", i))
-        if i + 2 < n_tiles:
-            out.append(("K", i + 2))
+def program(items, w):
+    """What the matrix warp of stream w does, in order: ("K" | "V", tile, used by this stream)."""
+    out, base = [], 0
+    for n, two in items:
+        mine = lambda i: two or (i & 1) == w
+        ahead = 1 if two else 2
+        out += [("K", base + i, mine(i)) for i in range(min(ahead, n))]
+        for i in range(n):
+            out.append(("V", base + i, mine(i)))
+            if i + ahead < n:
+                out.append(("K", base + i + ahead, mine(i + ahead)))
+        base += n
     return out
 
 
-@pytest.mark.parametrize("n_tiles", [1, 2, 3, 4, 5, 6, 17])
-def test_ring_positions(n_tiles):
-    """The positions the matrix-instruction warp computes, and that no load waits for a slot whose
-    release needs a later load."""
-    order = ring_order(n_tiles, False)
-    k_at = lambda i: i if i < 2 else 2 * i - 1
-    v_at = lambda i: 2 * i + 2 if i + 1 < n_tiles else 2 * i + 1
-    for i in range(n_tiles):
-        assert order[k_at(i)] == ("K", i) and order[v_at(i)] == ("V", i)
-    for two in (False, True):
-        order = ring_order(n_tiles, two)
-        # reads in program order of the issuing warp; a read releases its slot
-        reads = [("K", 0)] if two else [("K", i) for i in range(min(2, n_tiles))]
-        for i in range(n_tiles):
-            if two:
-                reads += [("V", i)] + ([("K", i + 1)] if i + 1 < n_tiles else [])
-            else:
-                reads += [("V", i)] + ([("K", i + 2)] if i + 2 < n_tiles else [])
-        for step, r in enumerate(reads):
-            assert order.index(r) <= step + SLOTS - 1
+@pytest.mark.parametrize("seed", range(40))
+def test_the_two_streams_never_wait_for_each_other_for_good(seed):
+    """Loads fill K slots and V slots in order; both streams give every tile back; a V product
+    waits for its stream's scores, which are there once they were issued.  Steps are taken in
+    random order: everything has to end, whoever runs ahead."""
+    rng = random.Random(seed)
+    its = [(rng.choice([1, 2, 3, 4, 5, 9]), rng.random() < 0.5) for _ in range(rng.randint(1, 6))]
+    total = sum(n for n, _ in its)
+    progs, at = [program(its, w) for w in range(2)], [0, 0]
+    loaded, given = {"K": 0, "V": 0}, {"K": [0] * total, "V": [0] * total}
+    slots = {"K": K_SLOTS, "V": V_SLOTS}
+    while at[0] < len(progs[0]) or at[1] < len(progs[1]):
+        moves = []
+        for kind in "KV":
+            f = loaded[kind]
+            if f < total and (f < slots[kind] or given[kind][f - slots[kind]] == 2):
+                moves.append(("load", kind))
+        for w in range(2):
+            if at[w] < len(progs[w]):
+                kind, tile, _ = progs[w][at[w]]
+                if tile < loaded[kind]:
+                    moves.append(("step", w))
+        assert moves, (its, at, loaded)
+        what, x = rng.choice(moves)
+        if what == "load":
+            loaded[x] += 1
+        else:
+            kind, tile, _ = progs[x][at[x]]
+            given[kind][tile] += 1
+            at[x] += 1
+    assert all(g == 2 for k in given.values() for g in k)
+    for w in range(2):                                   # every tile a stream owns: scores before values, once
+        for i in range(total):
+            steps = [j for j, (k, t, use) in enumerate(progs[w]) if t == i and use]
+            assert len(steps) in (0, 2) and (not steps or progs[w][steps[0]][0] == "K")
+    assert all(any(t == i and use for pr in progs for _, t, use in pr) for i in range(total))
