@@ -1457,7 +1457,7 @@ extern "C" int pkv_prompt_attention(int device, const pkv_prompt_args* a, void* 
   cfg.dynamicSmemBytes = pkv::kPaSmem;
   if (a->dtype == PKV_BF16) PKV_CUDA(cudaLaunchKernelEx(&cfg, pkv::prompt_attn_kernel<true>, qm, km, vm, p));
   else                      PKV_CUDA(cudaLaunchKernelEx(&cfg, pkv::prompt_attn_kernel<false>, qm, km, vm, p));
-  cfg.gridDim = dim3(sms - 1 > 0 ? sms - 1 : 1, 8);
+  cfg.gridDim = dim3(4 * sms);
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
   PKV_CUDA(cudaLaunchKernelEx(&cfg, pkv::prompt_join_kernel, p, sms));

@@ -230,6 +230,25 @@ __device__ __forceinline__ void store_row16(void* row, int out_dtype, int chunk,
   }
 }
 
+// Four neighbouring lanes, each with four pieces of its row: afterwards lane q of them holds piece q
+// of all four rows.  Two rounds of swaps.
+template <int N>
+__device__ __forceinline__ void quad_transpose(uint32_t (&pc)[4][N], int quad) {
+#pragma unroll
+  for (int d = 1; d <= 2; d <<= 1)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j & d) continue;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const uint32_t a = pc[j][e], b = pc[j | d][e];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, quad & d ? a : b, d);
+        pc[j][e] = quad & d ? got : a;
+        pc[j | d][e] = quad & d ? b : got;
+      }
+    }
+}
+
 template <bool BF16>
 __global__ void __launch_bounds__(kPaThreads, 1)
 prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
@@ -488,8 +507,20 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         const int prow = (two ? w * kPaRows : 0) + row;
         if (!whole) p.part_ml[(size_t)wk.slot * 256 + prow] = make_float2(m2, l);
         float4* po = p.part_o + (size_t)max(wk.slot, 0) * 32 * 256 + prow;
-        uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + orow * kHeadDim * (p.out_dtype == 4 ? 4 : 2);
-        const float* more = p.o_more ? p.o_more + orow * kHeadDim : nullptr;
+        // Written directly, a row is 256 bytes of its own: 32 lanes that store 16 bytes each of their
+        // rows touch 32 cache lines per instruction, and the store path takes one line a cycle (an
+        // item's epilogue took 5000 to 10000 cycles).  Four lanes swap pieces instead, so that
+        // each stores a quarter of the same 32 columns of four rows.
+        const bool wide = p.o_more != nullptr || p.out_dtype == 4;
+        const int quad = lane & 3;
+        int64_t qrow[4];
+        float qwb[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          qrow[i] = __shfl_sync(0xffffffffu, valid ? orow : (int64_t)-1, (lane & 28) + i);
+          qwb[i] = __shfl_sync(0xffffffffu, wb, (lane & 28) + i);
+        }
+        uint8_t* out = reinterpret_cast<uint8_t*>(p.out);
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
@@ -513,16 +544,39 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
             for (int i = 0; i < 8; ++i)
               po[(c * 8 + i) * 256] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
                                                   __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
-          } else if (valid) {
+          } else if (!wide) {
+            uint32_t pc[4][4];                                   // [piece of 8 columns][2 values each]
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float u = __uint_as_float(o[2 * i]) * wa, v = __uint_as_float(o[2 * i + 1]) * wa;
+              pc[i >> 2][i & 3] = p.out_dtype == 1 ? pack2<true>(u, v) : pack2<false>(u, v);
+            }
+            quad_transpose(pc, quad);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (qrow[i] >= 0)
+                *reinterpret_cast<uint4*>(out + qrow[i] * (kHeadDim * 2) + c * 64 + quad * 16) =
+                    make_uint4(pc[i][0], pc[i][1], pc[i][2], pc[i][3]);
+          } else {
+            uint32_t pc[4][8];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) pc[i >> 3][i & 7] = __float_as_uint(__uint_as_float(o[i]) * wa);
+            quad_transpose(pc, quad);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
+              if (qrow[i] < 0) continue;
               float v[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                v[e] = __uint_as_float(o[8 * i + e]) * wa;
-                if (more && wb != 0.f) v[e] = fmaf(more[c * 32 + i * 8 + e], wb, v[e]);
+              for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(pc[i][e]);
+              if (qwb[i] != 0.f) {
+                const float4* more = reinterpret_cast<const float4*>(p.o_more + qrow[i] * kHeadDim + c * 32 + quad * 8);
+                const float4 x = more[0], y = more[1];
+                v[0] = fmaf(x.x, qwb[i], v[0]); v[1] = fmaf(x.y, qwb[i], v[1]);
+                v[2] = fmaf(x.z, qwb[i], v[2]); v[3] = fmaf(x.w, qwb[i], v[3]);
+                v[4] = fmaf(y.x, qwb[i], v[4]); v[5] = fmaf(y.y, qwb[i], v[5]);
+                v[6] = fmaf(y.z, qwb[i], v[6]); v[7] = fmaf(y.w, qwb[i], v[7]);
               }
-              store_row16(dst, p.out_dtype, c * 4 + i, v);
+              store_row16(out + qrow[i] * kHeadDim * (p.out_dtype == 4 ? 4 : 2), p.out_dtype, c * 4 + quad, v);
             }
           }
         }
@@ -801,84 +855,95 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   }
 }
 
-// Adds up the pieces of the items that were cut, in the order of their keys.  Block (c, y):
-// the item in which CTA c's piece starts, if c is the first CTA to start inside it; one thread
-// per row, 16 of the 128 values.  The pieces are a few MB that were written a moment ago: L2.
+// Adds up the pieces of the items that were cut, in the order of their keys.  Every block reads
+// what each CTA did first (one record a thread), lists the items that were cut, and takes
+// tasks of (item, 8 of the 128 values); one thread per row, so a piece's values come in
+// 4 KB runs.  The pieces are a few MB that were written a moment ago: L2.
+constexpr int kPjTasks = 16;
 __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptParams p, int n_grid) {
+  __shared__ int64_t s_a[kPaMaxCtas];
+  __shared__ int s_kt0[kPaMaxCtas], s_kt1[kPaMaxCtas], s_n[kPaMaxCtas], s_head[kPaMaxCtas], s_last[kPaMaxCtas];
+  __shared__ int s_cnt[9];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int c = blockIdx.x + 1, row = threadIdx.x;
+  const int tid = threadIdx.x, row = tid;
   const int n_cta = p.rec[n_grid].kt0;
-  if (c >= n_cta) return;
-  const PromptRec r = p.rec[c];
-  if (!r.mid || r.kt0 >= r.n) return;                       // not inside an item, or all of it was done before
-  if (c > 1) {
-    const PromptRec b = p.rec[c - 1];
-    if (b.mid && b.a == r.a) return;                        // an earlier CTA starts inside it too
+  if (n_cta <= 1) return;
+  if (tid < n_cta) {
+    const PromptRec r = p.rec[tid];
+    s_a[tid] = r.mid ? r.a : -1;                            // -1: starts with an item of its own
+    s_kt0[tid] = r.kt0; s_kt1[tid] = r.kt1; s_n[tid] = r.n;
   }
-  if (r.kt0 == 0 && r.kt1 == r.n) return;                   // this CTA did all of it
-  int last = c;                                             // last CTA that starts inside the item
-  while (last + 1 < n_cta) {
-    const PromptRec b = p.rec[last + 1];
-    if (!b.mid || b.a != r.a) break;
-    if (b.kt0 == 0 && b.kt1 == b.n) return;
-    ++last;
-  }
-  const bool two = r.n_tok > p.tok_tile;
-  const int w = row >> 7, lr = row & 127;
-  if (w && !two) return;
-  const int tok_in = lr / p.group, head_in = lr - tok_in * p.group, tok = w * p.tok_tile + tok_in;
-  if (lr >= p.tok_tile * p.group || tok >= r.n_tok) return;
-  const int64_t orow = (int64_t)(r.q0 + tok) * p.n_q_heads + r.h * p.group + head_in;
-
-  // piece i: the CTA before c (its last item), then c .. last (their first items)
-  auto slot_of = [&](int i) { return i == 0 ? 2 * (c - 1) + 1 : 2 * (c + i - 1); };
-  auto has = [&](int i) {
-    if (i == 0) return r.kt0 > 0;
-    const PromptRec& b = p.rec[c + i - 1];
-    return b.kt1 > b.kt0;
-  };
-  const int n = last - c + 2;
-  float m = -INFINITY;
-  for (int i = 0; i < n; ++i)
-    if (has(i)) m = fmaxf(m, p.part_ml[(size_t)slot_of(i) * 256 + row].x);
-  float b2 = -INFINITY;
-  if (p.o_more) {
-    b2 = p.lse_more[orow] * 1.4426950408889634f;
-    m = fmaxf(m, b2);
-  }
-  float l = 0.f, acc[16];
-#pragma unroll
-  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-  for (int i = 0; i < n; ++i) {
-    if (!has(i)) continue;
-    const float2 ml = p.part_ml[(size_t)slot_of(i) * 256 + row];
-    const float f = ml.x == -INFINITY ? (ml.y == ml.y ? 0.f : ml.y) : exp2f(ml.x - m);
-    l += ml.y * f;
-    const float4* po = p.part_o + (size_t)slot_of(i) * 32 * 256 + row;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float4 v = po[(blockIdx.y * 4 + e) * 256];
-      acc[4 * e] += v.x * f; acc[4 * e + 1] += v.y * f; acc[4 * e + 2] += v.z * f; acc[4 * e + 3] += v.w * f;
+  __syncthreads();
+  // CTA c is the first to start inside an item that several CTAs share
+  bool head = false;
+  int last = tid;
+  if (tid > 0 && tid < n_cta && s_a[tid] >= 0 && s_a[tid - 1] != s_a[tid] && s_kt0[tid] < s_n[tid]) {
+    head = true;
+    for (int c = tid; c < n_cta && s_a[c] == s_a[tid]; ++c) {
+      if (s_kt0[c] == 0 && s_kt1[c] == s_n[c]) head = false;   // one CTA did all of it, and wrote it
+      last = c;
     }
   }
-  if (b2 != -INFINITY) {
-    const float f = exp2f(b2 - m);
-    l += f;
-    const float* more = p.o_more + orow * kHeadDim + blockIdx.y * 16;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) acc[e] = fmaf(more[e], f, acc[e]);
+  const unsigned mask = __ballot_sync(0xffffffffu, head);
+  if ((tid & 31) == 0) s_cnt[tid >> 5] = __popc(mask);
+  __syncthreads();
+  int at = __popc(mask & ((1u << (tid & 31)) - 1)), n_items = 0;
+  for (int w = 0; w < 8; ++w) {
+    if (w < (tid >> 5)) at += s_cnt[w];
+    n_items += s_cnt[w];
   }
-  const float inv = l > 0.f ? 1.f / l : (l != l ? l : 0.f);
-  uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + orow * kHeadDim * (p.out_dtype == 4 ? 4 : 2);
+  if (head) { s_head[at] = tid; s_last[at] = last; }
+  __syncthreads();
+
+  for (int task = blockIdx.x; task < n_items * kPjTasks; task += gridDim.x) {
+    const int c = s_head[task / kPjTasks], col = task % kPjTasks, end = s_last[task / kPjTasks];
+    const int q0 = p.rec[c].q0, n_tok = p.rec[c].n_tok, h = p.rec[c].h;
+    const bool two = n_tok > p.tok_tile;
+    const int w = row >> 7, lr = row & 127;
+    const int tok_in = lr / p.group, tok = w * p.tok_tile + tok_in;
+    if ((w && !two) || lr >= p.tok_tile * p.group || tok >= n_tok) continue;
+    const int64_t orow = (int64_t)(q0 + tok) * p.n_q_heads + h * p.group + (lr - tok_in * p.group);
+    // piece c - 1 .. end: the last item of CTA c - 1, the first item of the others; some are empty
+    auto slot_of = [&](int i) { return i < c ? 2 * i + 1 : 2 * i; };
+    auto has = [&](int i) { return i < c ? s_kt0[c] > 0 : s_kt1[i] > s_kt0[i]; };
+    float m = -INFINITY;
+#pragma unroll 4
+    for (int i = c - 1; i <= end; ++i)
+      if (has(i)) m = fmaxf(m, p.part_ml[(size_t)slot_of(i) * 256 + row].x);
+    float b2 = -INFINITY;
+    if (p.o_more) {
+      b2 = p.lse_more[orow] * 1.4426950408889634f;
+      m = fmaxf(m, b2);
+    }
+    float l = 0.f, acc[8];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    float v[8];
+    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+#pragma unroll 4
+    for (int i = c - 1; i <= end; ++i) {
+      if (!has(i)) continue;
+      const float2 ml = p.part_ml[(size_t)slot_of(i) * 256 + row];
+      const float4* po = p.part_o + (size_t)slot_of(i) * 32 * 256 + (size_t)col * 2 * 256 + row;
+      const float4 x = po[0], y = po[256];
+      const float f = ml.x == -INFINITY ? (ml.y == ml.y ? 0.f : ml.y) : exp2f(ml.x - m);
+      l += ml.y * f;
+      acc[0] += x.x * f; acc[1] += x.y * f; acc[2] += x.z * f; acc[3] += x.w * f;
+      acc[4] += y.x * f; acc[5] += y.y * f; acc[6] += y.z * f; acc[7] += y.w * f;
+    }
+    if (b2 != -INFINITY) {
+      const float f = exp2f(b2 - m);
+      l += f;
+      const float* more = p.o_more + orow * kHeadDim + col * 8;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = acc[8 * k + e] * inv;
-    store_row16(dst, p.out_dtype, blockIdx.y * 2 + k, v);
+      for (int e = 0; e < 8; ++e) acc[e] = fmaf(more[e], f, acc[e]);
+    }
+    const float inv = l > 0.f ? 1.f / l : (l != l ? l : 0.f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= inv;
+    uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + orow * kHeadDim * (p.out_dtype == 4 ? 4 : 2);
+    store_row16(dst, p.out_dtype, col, acc);
+    if (p.lse && col == 0)
+      p.lse[orow] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : (l != l ? l : -INFINITY);
   }
-  if (p.lse && blockIdx.y == 0)
-    p.lse[orow] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : (l != l ? l : -INFINITY);
 }
 
 }  // namespace pkv
