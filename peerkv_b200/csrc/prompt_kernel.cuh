@@ -52,7 +52,7 @@ constexpr int kPaMaxCtas = 256;
 constexpr int kPaSoftmaxRegs = 208;
 constexpr int kPaOtherRegs = 80;
 constexpr uint32_t kPaColO = 256;                        // TMEM columns: S0 0, S1 128, O0 256, O1 384
-constexpr int kPaItemCost = 192;   // what an item costs besides its keys, in keys
+constexpr int kPaItemCost = 384;   // what an item costs besides its keys, in keys
 constexpr int kPaMinPiece = 512;   // no CTA gets less than this many keys of work
 
 // Which CTA found which item cut (one per CTA, for the join).
@@ -118,6 +118,11 @@ __device__ __forceinline__ int64_t prompt_items_cost(const PromptSeq& s, int64_t
   return t * s.add + s.step * (t * (t + 1) / 2);
 }
 
+// (One copy: inlined everywhere, 64-bit divisions and waits had grown the kernel to 160 KB, more
+// than the instruction cache holds, and each item's first tile and epilogue ran at the speed of
+// the cache behind it.)
+__device__ __noinline__ int64_t prompt_div(int64_t a, int64_t b) { return a / b; }
+
 struct PromptItem {
   int s, h, t;                 // sequence, kv-head, item of the sequence
   int64_t a, x0, x1;           // item's start on the cost axis; this CTA's piece of the axis
@@ -128,7 +133,7 @@ struct PromptItem {
 
   // piece of a CTA -> tile index: monotone, 0 at the item's start, n at its end
   __device__ __forceinline__ int cut(int64_t y, int64_t cost) const {
-    return y <= 0 ? 0 : y >= cost ? n : (int)(y * n / cost);
+    return y <= 0 ? 0 : y >= cost ? n : (int)prompt_div(y * n, cost);
   }
   __device__ __forceinline__ void fill(const PromptParams& p) {
     const int tt = 2 * p.tok_tile;
@@ -140,11 +145,11 @@ struct PromptItem {
     kt0 = cut(x0 - a, cost);
     kt1 = cut(x1 - a, cost);
   }
-  // first item of the piece: s and `base` (cost before sequence s) are known
+  // first item of the piece (fill() follows): s and `base`, the cost before sequence s, are known
   __device__ __forceinline__ void start(const PromptParams& p, int64_t base) {
     seq = prompt_seq(p, s);
     const int64_t per = prompt_items_cost(seq, seq.tiles);
-    h = (int)((x0 - base) / per);
+    h = (int)prompt_div(x0 - base, per);
     const int64_t y = x0 - base - h * per;
     int lo = 0, hi = seq.tiles - 1;                      // largest t with cost(0 .. t-1) <= y
     while (lo < hi) {
@@ -153,9 +158,8 @@ struct PromptItem {
     }
     t = lo;
     a = base + h * per + prompt_items_cost(seq, t);
-    fill(p);
   }
-  // the next item; false when the piece is done
+  // the next item (fill() follows); false when the piece is done
   __device__ __forceinline__ bool next(const PromptParams& p) {
     a += seq.add + seq.step * (t + 1);
     if (a >= x1) return false;
@@ -169,7 +173,6 @@ struct PromptItem {
         } while (seq.tiles == 0);
       }
     }
-    fill(p);
     return true;
   }
   // this CTA has tiles of the item, or the item has none and starts here
@@ -194,17 +197,18 @@ constexpr int kPaWorkRing = 4;
 // A step of the pipeline takes microseconds; a wait that has not ended after two seconds sets
 // the abort flag, every later wait returns at once, and the CTA runs out.
 __device__ __forceinline__ bool pa_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {   // whole warp
-  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   unsigned long long t0 = 0;
-  for (uint32_t w = 0;; ++w) {       // every exit is taken by all lanes together
-    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    if (__any_sync(0xffffffffu, *abort_flag)) return false;
-    if ((w & 63u) == 63u) {
-      const unsigned long long now = global_ns();
-      if (t0 == 0) t0 = now;
-      if (__any_sync(0xffffffffu, now - t0 > 2000000000ull)) { *abort_flag = 1; return false; }
+#pragma unroll 1
+  for (uint32_t w = 1; !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)); ++w) {   // all lanes leave together
+    if (w & 63u) continue;                            // the clock is slow to read
+    const unsigned long long now = global_ns();
+    if (t0 == 0) t0 = now;
+    if (__any_sync(0xffffffffu, *abort_flag || now - t0 > 2000000000ull)) {
+      *abort_flag = 1;
+      return false;
     }
   }
+  return true;
 }
 
 // The same value in every lane, in a form in which the compiler knows it.
@@ -312,13 +316,15 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   __syncthreads();
   tc_fence_after();
   int64_t before = incl - mine, total = 0;
+#pragma unroll 1
   for (int w = 0; w < kPaThreads / 32; ++w) {
     if (w < warp) before += wsum[w];
     total += wsum[w];
   }
-  const int n_cta = (int)min((int64_t)gridDim.x, (total + kPaMinPiece - 1) / kPaMinPiece);
+  const int n_cta = (int)min((int64_t)gridDim.x, prompt_div(total + kPaMinPiece - 1, kPaMinPiece));
   const bool active = (int)blockIdx.x < n_cta;
-  const int64_t x0 = active ? total * blockIdx.x / n_cta : 0, x1 = active ? total * (blockIdx.x + 1) / n_cta : 0;
+  const int64_t x0 = active ? prompt_div(total * blockIdx.x, n_cta) : 0;
+  const int64_t x1 = active ? prompt_div(total * (blockIdx.x + 1), n_cta) : 0;
   if (active && before <= x0 && x0 < before + mine) {
     int64_t base = before;
     for (int s = sb; s < se; ++s) {
@@ -377,17 +383,6 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
             for (int i = 0; i < 32; ++i)
               if (c * 32 + i >= left) sreg[c][i] = 0xff800000u;           // -inf
         }
-        auto row_max = [&]() {
-          float mx[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            mx[c] = fmaxf(__uint_as_float(sreg[c][0]), __uint_as_float(sreg[c][1]));
-#pragma unroll
-            for (int i = 2; i < 32; i += 2)
-              mx[c] = max3(mx[c], __uint_as_float(sreg[c][i]), __uint_as_float(sreg[c][i + 1]));
-          }
-          return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        };
         const uint64_t sl2 = pack_f32x2(sl, sl);
         uint64_t ref2, sum_a, sum_b;                                       // two fp32 sums each
         // a row that has seen no key yet has m = -inf: 0 as the reference keeps exp2(-inf) = 0
@@ -421,31 +416,31 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           if (lane == 0) mbar_arrive(p_full(2 * w + half));
         };
         // The exponentials start with the reference of the tiles before, beside the search for this
-        // tile's maximum; only if that lies more than 2^8 above are they done again.
-        if (j == 0) m = row_max();
-        set_ref();
-        exps(0, true);
-        const float tile_max = fmaxf(mx0, mx1);
-        if (__any_sync(0xffffffffu, (tile_max - m) * sl > 8.f)) {
+        // tile's maximum; only if that lies more than 2^8 above are they done again (as they are
+        // for an item's first tile, which has no reference yet).
+#pragma unroll 1
+        for (;;) {
+          set_ref();
+          mx0 = mx1 = -INFINITY;
+          exps(0, true);
+          const float tile_max = fmaxf(mx0, mx1);
+          if (!__any_sync(0xffffffffu, (tile_max - m) * sl > 8.f)) break;
           // The product that wrote O last is complete: the scores just waited for were issued
           // behind it, and the next one waits for this warpgroup.
           const float mn = fmaxf(m, tile_max);
           const float alpha = m == -INFINITY ? 0.f : fast_exp2((m - mn) * sl);
           l *= alpha;
           m = mn;
-          set_ref();
-          if (j > 0) {
+          if (j == 0) continue;
 #pragma unroll 1
-            for (int c = 0; c < 8; ++c) {
-              uint32_t o[16];
-              tmem_ld16(o, to + c * 16);
-              tmem_wait_ld();
+          for (int c = 0; c < 8; ++c) {
+            uint32_t o[16];
+            tmem_ld16(o, to + c * 16);
+            tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tmem_st16(to + c * 16, o);
-            }
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st16(to + c * 16, o);
           }
-          exps(0, false);
         }
         hand_over(0);
         exps(1, false);
@@ -507,76 +502,100 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         const int prow = (two ? w * kPaRows : 0) + row;
         if (!whole) p.part_ml[(size_t)wk.slot * 256 + prow] = make_float2(m2, l);
         float4* po = p.part_o + (size_t)max(wk.slot, 0) * 32 * 256 + prow;
-        // Written directly, a row is 256 bytes of its own: 32 lanes that store 16 bytes each of their
-        // rows touch 32 cache lines per instruction, and the store path takes one line a cycle (an
-        // item's epilogue took 5000 to 10000 cycles).  Four lanes swap pieces instead, so that
-        // each stores a quarter of the same 32 columns of four rows.
-        const bool wide = p.o_more != nullptr || p.out_dtype == 4;
-        const int quad = lane & 3;
-        int64_t qrow[4];
-        float qwb[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          qrow[i] = __shfl_sync(0xffffffffu, valid ? orow : (int64_t)-1, (lane & 28) + i);
-          qwb[i] = __shfl_sync(0xffffffffu, wb, (lane & 28) + i);
-        }
-        uint8_t* out = reinterpret_cast<uint8_t*>(p.out);
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t o[32];
-          if (steps > 0) {
-            tmem_ld32(o, to + c * 32);
-            tmem_wait_ld();
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = 0u;
-          }
+        // 16 columns of this row's O, of both streams where they share the row tile
+        auto columns = [&](uint32_t (&o)[16], int col) {
+          tmem_ld16(o, to + col);
           if (join) {
-            uint32_t o1[32];
-            tmem_ld32(o1, to + 128 + c * 32);
+            uint32_t o1[16];
+            tmem_ld16(o1, to + 128 + col);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
+            for (int i = 0; i < 16; ++i)
               o[i] = __float_as_uint(__uint_as_float(o[i]) * a0 + __uint_as_float(o1[i]) * a1);
           }
-          if (!whole) {
+          tmem_wait_ld();
+          if (steps == 0) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              po[(c * 8 + i) * 256] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                                  __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
-          } else if (!wide) {
-            uint32_t pc[4][4];                                   // [piece of 8 columns][2 values each]
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float u = __uint_as_float(o[2 * i]) * wa, v = __uint_as_float(o[2 * i + 1]) * wa;
-              pc[i >> 2][i & 3] = p.out_dtype == 1 ? pack2<true>(u, v) : pack2<false>(u, v);
-            }
-            quad_transpose(pc, quad);
+            for (int i = 0; i < 16; ++i) o[i] = 0u;
+          }
+        };
+        if (!whole) {
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {
+            uint32_t o[16];
+            columns(o, c * 16);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (qrow[i] >= 0)
-                *reinterpret_cast<uint4*>(out + qrow[i] * (kHeadDim * 2) + c * 64 + quad * 16) =
-                    make_uint4(pc[i][0], pc[i][1], pc[i][2], pc[i][3]);
-          } else {
-            uint32_t pc[4][8];
+              po[(c * 4 + i) * 256] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                                  __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+          }
+        } else {
+          // Written directly, a row is 256 bytes of its own: 32 lanes that store 16 bytes each of their
+          // rows touch 32 cache lines per instruction, and the store path takes about three
+          // cycles a line (an item's epilogue took 5000 to 10000 cycles).  Four lanes swap pieces
+          // first, so that a line is touched for 64 bytes at a time.
+          const int quad = lane & 3;
+          int64_t qrow[4];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) pc[i >> 3][i & 7] = __float_as_uint(__uint_as_float(o[i]) * wa);
-            quad_transpose(pc, quad);
+          for (int i = 0; i < 4; ++i) qrow[i] = __shfl_sync(0xffffffffu, valid ? orow : (int64_t)-1, (lane & 28) + i);
+          if (!p.o_more && p.out_dtype != 4) {
+            uint4* dst[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (qrow[i] < 0) continue;
-              float v[8];
+            for (int i = 0; i < 4; ++i) dst[i] = static_cast<uint4*>(p.out) + qrow[i] * (kHeadDim / 8) + quad;
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t pc[4][4];                                 // [piece of 8 columns][2 values each]
 #pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(pc[i][e]);
-              if (qwb[i] != 0.f) {
-                const float4* more = reinterpret_cast<const float4*>(p.o_more + qrow[i] * kHeadDim + c * 32 + quad * 8);
-                const float4 x = more[0], y = more[1];
-                v[0] = fmaf(x.x, qwb[i], v[0]); v[1] = fmaf(x.y, qwb[i], v[1]);
-                v[2] = fmaf(x.z, qwb[i], v[2]); v[3] = fmaf(x.w, qwb[i], v[3]);
-                v[4] = fmaf(y.x, qwb[i], v[4]); v[5] = fmaf(y.y, qwb[i], v[5]);
-                v[6] = fmaf(y.z, qwb[i], v[6]); v[7] = fmaf(y.w, qwb[i], v[7]);
+              for (int k = 0; k < 2; ++k) {
+                uint32_t o[16];
+                columns(o, c * 32 + k * 16);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const float u = __uint_as_float(o[2 * i]) * wa, v = __uint_as_float(o[2 * i + 1]) * wa;
+                  pc[2 * k + (i >> 2)][i & 3] = p.out_dtype == 1 ? pack2<true>(u, v) : pack2<false>(u, v);
+                }
               }
-              store_row16(out + qrow[i] * kHeadDim * (p.out_dtype == 4 ? 4 : 2), p.out_dtype, c * 4 + quad, v);
+              quad_transpose(pc, quad);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if (qrow[i] >= 0) *dst[i] = make_uint4(pc[i][0], pc[i][1], pc[i][2], pc[i][3]);
+                dst[i] += 4;
+              }
+            }
+          } else {
+            float qwb[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) qwb[i] = __shfl_sync(0xffffffffu, wb, (lane & 28) + i);
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+              uint32_t pc[4][4];                                 // [piece of 4 columns]
+              columns(reinterpret_cast<uint32_t(&)[16]>(pc), c * 16);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) pc[i >> 2][i & 3] = __float_as_uint(__uint_as_float(pc[i >> 2][i & 3]) * wa);
+              quad_transpose(pc, quad);
+              float4 x[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (qwb[i] != 0.f && qrow[i] >= 0)
+                  x[i] = *reinterpret_cast<const float4*>(p.o_more + qrow[i] * kHeadDim + c * 16 + quad * 4);
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if (qrow[i] < 0) continue;
+                const int64_t at = qrow[i] * kHeadDim + c * 16 + quad * 4;
+                const float4 v = make_float4(fmaf(x[i].x, qwb[i], __uint_as_float(pc[i][0])),
+                                             fmaf(x[i].y, qwb[i], __uint_as_float(pc[i][1])),
+                                             fmaf(x[i].z, qwb[i], __uint_as_float(pc[i][2])),
+                                             fmaf(x[i].w, qwb[i], __uint_as_float(pc[i][3])));
+                const bool bf = p.out_dtype == 1;
+                if (p.out_dtype == 4)
+                  *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = v;
+                else
+                  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at) =
+                      make_uint2(bf ? pack2<true>(v.x, v.y) : pack2<false>(v.x, v.y),
+                                 bf ? pack2<true>(v.z, v.w) : pack2<false>(v.z, v.w));
+              }
             }
           }
         }
@@ -602,6 +621,10 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       uint32_t n_tile = 0, n_q = 0;                       // tiles and Q loads issued
       bool ok = active;
       PromptItem it;
+      it.s = -1;
+      it.x0 = x0;
+      it.x1 = x1;
+      bool recorded = false;
       uint32_t n_given = 0;
       // the work list: what this warp puts into the ring the other warps take out
       auto give = [&](const PromptWork& v) {
@@ -616,21 +639,24 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       };
       auto make = [&]() {
         bool have = true;
-        if (n_given == 0) {
-          it.x0 = x0;
-          it.x1 = x1;
-          it.s = (int)first[0];
-          it.start(p, first[1]);
+        do {
+          if (it.s < 0) {
+            it.s = (int)first[0];
+            it.start(p, first[1]);
+          } else {
+            have = it.next(p);
+          }
+          if (have) it.fill(p);
+        } while (have && !it.mine() && recorded);
+        if (!recorded) {                             // what the join needs of the first item
+          recorded = true;
           if (lane == 0) {
             PromptRec r;
             r.a = it.a; r.mid = it.x0 > it.a ? 1 : 0; r.kt0 = it.kt0; r.kt1 = it.kt1; r.n = it.n;
             r.q0 = it.q0; r.n_tok = it.n_tok; r.h = it.h; r.pad = 0;
             p.rec[blockIdx.x] = r;
           }
-        } else {
-          have = it.next(p);
         }
-        while (have && !it.mine()) have = it.next(p);
         wk.n_tiles = have ? it.kt1 - it.kt0 : -1;
         wk.kt0 = it.kt0; wk.vis = it.vis; wk.len = it.seq.len;
         wk.lim0 = it.seq.len - it.seq.n + (it.q0 - it.seq.q0) + 1;
@@ -650,6 +676,7 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           if (elect_one()) {
             const uint32_t half = (uint32_t)p.tok_tile * p.group * 128u;
             mbar_arrive_expect_tx(q_full, half * (two ? 4u : 2u));
+#pragma unroll 1
             for (int w = 0; w < (two ? 2 : 1); ++w)
               for (int d = 0; d < 2; ++d)
                 tma_load_3d(smem + w * kPaTileBytes + d * kPaHalfBytes, &qmap, q_full, d * 64, h * p.group,
@@ -684,6 +711,7 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
             }
           } else {
             int tok = key0 % p.page_size;
+#pragma unroll 1
             for (int b = 0; b < n_box; ++b) {
               const int pg = uniform(__shfl_sync(0xffffffffu, page, b));
               const int c1 = p.head_major ? tok : h, c2 = p.head_major ? h : tok;
@@ -700,6 +728,7 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           return true;
         };
         int p0 = fetch(0), p1 = fetch(1), p2 = fetch(2);
+#pragma unroll 1
         for (int i = 0; i < n_tiles && ok; ++i) {
           ok = load(i, p0);
           p0 = p1;
@@ -751,9 +780,12 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           if (elect_one()) {
             if (ksteps == 8) {
 #pragma unroll
-              for (int ks = 4 * half; ks < 4 * half + 4; ++ks)
+              for (int k = 0; k < 4; ++k) {
+                const int ks = 4 * half + k;
                 umma_ts(tm + kPaColO + w * 128, tm + w * 128 + ks * 8, va + ks * 128, hi, idesc_pv, ks > 0 ? 1u : keep);
+              }
             } else {
+#pragma unroll 1
               for (int ks = 4 * half; ks < min(4 * half + 4, ksteps); ++ks)
                 umma_ts(tm + kPaColO + w * 128, tm + w * 128 + ks * 8, va + ks * 128, hi, idesc_pv, ks > 0 ? 1u : keep);
             }
@@ -767,6 +799,7 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       auto clean = [&](uint32_t i, int kt, int ksteps) {
         const int from = wk.len - kt * kPaKeys, to = ksteps * 16;
         uint8_t* v = sgen + kPaRingOff + pa_slot(1, i) * kPaTileBytes;
+#pragma unroll 1
         for (int r = max(from, 0); r < to; ++r) {
           *reinterpret_cast<uint32_t*>(v + r * 128 + lane * 4) = 0u;
           *reinterpret_cast<uint32_t*>(v + kPaHalfBytes + r * 128 + lane * 4) = 0u;
@@ -793,51 +826,44 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           give_back(1, base + i);
           return true;
         };
+        auto pass = [&](int kv, int i) {
+          if (!wait_tile(kv, base + i)) return false;
+          if (elect_one()) mbar_arrive(empty(pa_slot(kv, base + i)));
+          __syncwarp();
+          return true;
+        };
         auto scores = [&](int i, int qtile) {
           if (!wait_tile(0, base + i)) return false;
           qk(qtile, base + i);
           give_back(0, base + i);
           return true;
         };
-        if (uniform(wk.two)) {
-          // Both streams take every tile, and they issue in turn: O_0 (+)= P_0 V and the next S_0, then
-          // the same of stream 1.  Left alone they fall into step, and the exponentials of both
-          // wait for the tensor cores and then compete (measured: 4300 cycles a step instead of
-          // 3100).
-          auto pass_turn = [&]() { if (elect_one()) mbar_arrive(turn(w ^ 1)); __syncwarp(); };
-          ok = scores(0, w);
-          if (n_tiles == 1) commit(q_empty);
-          for (int j = 0; j < n_tiles && ok; ++j) {
-            if (!(ok = values(j, j == 0, true))) break;
-            if (j + 1 == n_tiles) {
-              commit(o_full(w));
-            } else {
-              ok = scores(j + 1, w);
-              if (j + 2 == n_tiles) commit(q_empty);
+        // Two row tiles: both streams take every tile, and they issue in turn: O_0 (+)= P_0 V and the
+        // next S_0, then the same of stream 1.  Left alone they fall into step, and the
+        // exponentials of both wait for the tensor cores and then compete (measured: 4300 cycles a
+        // step instead of 3100).  One row tile: stream w takes tiles w, w + 2, ..., and lets the
+        // others pass, so that no slot is filled again before both have seen it.
+        const bool two = uniform(wk.two);
+        const int ahead = two ? 1 : 2;                  // scores a stream is ahead of its values
+#pragma unroll 1
+        for (int t = 0; t < n_tiles + ahead; ++t) {
+          const int i = t - ahead;
+          const bool mine = two || (t & 1) == w;        // of tile t and, ahead being 1 or 2, of tile i
+          if (i >= 0) {
+            if (mine) {
+              if (!(ok = values(i, i < (two ? 1 : 2), two))) break;
+              if (i + (two ? 1 : 2) >= n_tiles) commit(o_full(w));
+            } else if (!(ok = pass(1, i))) {
+              break;
             }
-            pass_turn();
           }
-        } else {
-          // one row tile: stream w takes tiles w, w + 2, ..., and lets the others pass, so that no
-          // slot is filled again before both have seen it
-          auto pass = [&](int kv, int i) {
-            if (!wait_tile(kv, base + i)) return false;
-            if (elect_one()) mbar_arrive(empty(pa_slot(kv, base + i)));
+          if (t < n_tiles) {
+            if (!(ok = mine ? scores(t, two ? w : 0) : pass(0, t))) break;
+            if (t + 1 == n_tiles) commit(q_empty);
+          }
+          if (two && i >= 0) {
+            if (elect_one()) mbar_arrive(turn(w ^ 1));
             __syncwarp();
-            return true;
-          };
-          ok = w == 0 ? scores(0, 0) : pass(0, 0);
-          if (ok && n_tiles > 1) ok = w == 1 ? scores(1, 0) : pass(0, 1);
-          if (n_tiles <= 2) commit(q_empty);
-          for (int i = 0; i < n_tiles && ok; ++i) {
-            const bool mine = (i & 1) == w;
-            if (!(ok = mine ? values(i, i < 2, false) : pass(1, i))) break;
-            if (i + 2 < n_tiles) {
-              ok = mine ? scores(i + 2, 0) : pass(0, i + 2);
-              if (i + 3 == n_tiles) commit(q_empty);
-            } else if (mine) {
-              commit(o_full(w));
-            }
           }
         }
       }
