@@ -118,10 +118,11 @@ __device__ __forceinline__ int64_t prompt_items_cost(const PromptSeq& s, int64_t
   return t * s.add + s.step * (t * (t + 1) / 2);
 }
 
-// (One copy: inlined everywhere, 64-bit divisions and waits had grown the kernel to 160 KB, more
-// than the instruction cache holds, and each item's first tile and epilogue ran at the speed of
-// the cache behind it.)
-__device__ __noinline__ int64_t prompt_div(int64_t a, int64_t b) { return a / b; }
+// Where CTA c's piece of the cost axis starts.  All CTAs compute it alike, so it may be rounded as it
+// likes as long as it ascends; a 64-bit integer division costs some 300 cycles of the start.
+__device__ __forceinline__ int64_t prompt_cut(int64_t total, int c, int n_cta, double inv) {
+  return c >= n_cta ? total : (int64_t)((double)(total * c) * inv);
+}
 
 struct PromptItem {
   int s, h, t;                 // sequence, kv-head, item of the sequence
@@ -133,7 +134,8 @@ struct PromptItem {
 
   // piece of a CTA -> tile index: monotone, 0 at the item's start, n at its end
   __device__ __forceinline__ int cut(int64_t y, int64_t cost) const {
-    return y <= 0 ? 0 : y >= cost ? n : (int)prompt_div(y * n, cost);
+    if (y <= 0 || n == 0) return 0;
+    return y >= cost ? n : min(n, (int)((float)y * __fdividef((float)n, (float)cost)));
   }
   __device__ __forceinline__ void fill(const PromptParams& p) {
     const int tt = 2 * p.tok_tile;
@@ -145,11 +147,13 @@ struct PromptItem {
     kt0 = cut(x0 - a, cost);
     kt1 = cut(x1 - a, cost);
   }
-  // first item of the piece (fill() follows): s and `base`, the cost before sequence s, are known
+  // first item of the piece (fill() follows): s, seq and `base`, the cost before s, are known
   __device__ __forceinline__ void start(const PromptParams& p, int64_t base) {
-    seq = prompt_seq(p, s);
     const int64_t per = prompt_items_cost(seq, seq.tiles);
-    h = (int)prompt_div(x0 - base, per);
+    h = (int)((float)(x0 - base) / (float)per);          // about; the next lines make it exact
+    h = min(max(h, 0), p.n_kv_heads - 1);
+    while (h > 0 && h * per > x0 - base) --h;
+    while (h + 1 < p.n_kv_heads && (h + 1) * per <= x0 - base) ++h;
     const int64_t y = x0 - base - h * per;
     int lo = 0, hi = seq.tiles - 1;                      // largest t with cost(0 .. t-1) <= y
     while (lo < hi) {
@@ -279,7 +283,9 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   volatile int64_t* first = reinterpret_cast<volatile int64_t*>(misc + 280);   // s, base
   int64_t* wsum = reinterpret_cast<int64_t*>(misc + 296);                      // 12 warp sums
   PromptWork* ring = reinterpret_cast<PromptWork*>(misc + 400);                // 4 x 48 bytes
-  float2* xml = reinterpret_cast<float2*>(misc + 640);                         // [128] (m, l) of stream 1
+  float2* xml = reinterpret_cast<float2*>(misc + 640);                         // behind the first sequence at 592
+  static_assert(sizeof(PromptSeq) <= 48, "first sequence");
+
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kPaSlots; ++i) { mbar_init(full(i), 1); mbar_init(empty(i), 2); }
@@ -301,9 +307,10 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   const int per_thread = (p.n_seq + kPaThreads - 1) / kPaThreads;
   const int sb = min((int)threadIdx.x * per_thread, p.n_seq), se = min(sb + per_thread, p.n_seq);
   int64_t mine = 0;
+  PromptSeq seq;
   for (int s = sb; s < se; ++s) {
-    const PromptSeq q = prompt_seq(p, s);
-    mine += p.n_kv_heads * prompt_items_cost(q, q.tiles);
+    seq = prompt_seq(p, s);
+    mine += p.n_kv_heads * prompt_items_cost(seq, seq.tiles);
   }
   int64_t incl = mine;
 #pragma unroll
@@ -321,16 +328,22 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     if (w < warp) before += wsum[w];
     total += wsum[w];
   }
-  const int n_cta = (int)min((int64_t)gridDim.x, prompt_div(total + kPaMinPiece - 1, kPaMinPiece));
+  const int n_cta = (int)min((int64_t)gridDim.x, (total + kPaMinPiece - 1) / kPaMinPiece);
   const bool active = (int)blockIdx.x < n_cta;
-  const int64_t x0 = active ? prompt_div(total * blockIdx.x, n_cta) : 0;
-  const int64_t x1 = active ? prompt_div(total * (blockIdx.x + 1), n_cta) : 0;
+  const double inv = active ? 1.0 / n_cta : 0.0;
+  const int64_t x0 = active ? prompt_cut(total, blockIdx.x, n_cta, inv) : 0;
+  const int64_t x1 = active ? prompt_cut(total, blockIdx.x + 1, n_cta, inv) : 0;
   if (active && before <= x0 && x0 < before + mine) {
     int64_t base = before;
     for (int s = sb; s < se; ++s) {
-      const PromptSeq q = prompt_seq(p, s);
-      const int64_t c = p.n_kv_heads * prompt_items_cost(q, q.tiles);
-      if (x0 < base + c) { first[0] = s; first[1] = base; break; }
+      if (se - sb > 1) seq = prompt_seq(p, s);
+      const int64_t c = p.n_kv_heads * prompt_items_cost(seq, seq.tiles);
+      if (x0 < base + c) {
+        first[0] = s;
+        first[1] = base;
+        *reinterpret_cast<PromptSeq*>(misc + 592) = seq;
+        break;
+      }
       base += c;
     }
   }
@@ -642,6 +655,7 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         do {
           if (it.s < 0) {
             it.s = (int)first[0];
+            it.seq = *reinterpret_cast<const PromptSeq*>(misc + 592);
             it.start(p, first[1]);
           } else {
             have = it.next(p);
@@ -886,17 +900,20 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
 // tasks of (item, 8 of the 128 values); one thread per row, so a piece's values come in
 // 4 KB runs.  The pieces are a few MB that were written a moment ago: L2.
 constexpr int kPjTasks = 16;
+constexpr int kPjBatch = 8;        // pieces in flight per thread: a join is a few trips to the L2, not one per piece
 __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptParams p, int n_grid) {
   __shared__ int64_t s_a[kPaMaxCtas];
-  __shared__ int s_kt0[kPaMaxCtas], s_kt1[kPaMaxCtas], s_n[kPaMaxCtas], s_head[kPaMaxCtas], s_last[kPaMaxCtas];
-  __shared__ int s_cnt[9];
+  __shared__ int s_kt0[kPaMaxCtas], s_kt1[kPaMaxCtas], s_n[kPaMaxCtas];
+  __shared__ int4 s_item[kPaMaxCtas];                      // first row, tokens, kv-head, first entry of its list
+  __shared__ int s_count[kPaMaxCtas], s_slot[2 * kPaMaxCtas], s_cnt[8];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tid = threadIdx.x, row = tid;
+  PromptRec r;
+  if (tid < n_grid) r = p.rec[tid];                        // (only those of the first n_cta are this launch's)
   const int n_cta = p.rec[n_grid].kt0;
   if (n_cta <= 1) return;
   if (tid < n_cta) {
-    const PromptRec r = p.rec[tid];
-    s_a[tid] = r.mid ? r.a : -1;                            // -1: starts with an item of its own
+    s_a[tid] = r.mid ? r.a : -1;                           // -1: starts with an item of its own
     s_kt0[tid] = r.kt0; s_kt1[tid] = r.kt1; s_n[tid] = r.n;
   }
   __syncthreads();
@@ -918,49 +935,69 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptParams p, 
     if (w < (tid >> 5)) at += s_cnt[w];
     n_items += s_cnt[w];
   }
-  if (head) { s_head[at] = tid; s_last[at] = last; }
+  if (head) {
+    // the item's pieces in order: the last item of CTA tid - 1, the first items of tid .. last,
+    // those that are not empty.  Lists cannot overlap: an item has at most last - tid + 2 entries
+    int e = tid + at;
+    s_item[at] = make_int4(r.q0, r.n_tok, r.h, e);
+    if (s_kt0[tid] > 0) s_slot[e++] = 2 * (tid - 1) + 1;
+    for (int c = tid; c <= last; ++c)
+      if (s_kt1[c] > s_kt0[c]) s_slot[e++] = 2 * c;
+    s_count[at] = e - (tid + at);
+  }
   __syncthreads();
 
   for (int task = blockIdx.x; task < n_items * kPjTasks; task += gridDim.x) {
-    const int c = s_head[task / kPjTasks], col = task % kPjTasks, end = s_last[task / kPjTasks];
-    const int q0 = p.rec[c].q0, n_tok = p.rec[c].n_tok, h = p.rec[c].h;
-    const bool two = n_tok > p.tok_tile;
+    const int4 item = s_item[task / kPjTasks];
+    const int col = task % kPjTasks, n = s_count[task / kPjTasks];
+    const int* slots = s_slot + item.w;
     const int w = row >> 7, lr = row & 127;
     const int tok_in = lr / p.group, tok = w * p.tok_tile + tok_in;
-    if ((w && !two) || lr >= p.tok_tile * p.group || tok >= n_tok) continue;
-    const int64_t orow = (int64_t)(q0 + tok) * p.n_q_heads + h * p.group + (lr - tok_in * p.group);
-    // piece c - 1 .. end: the last item of CTA c - 1, the first item of the others; some are empty
-    auto slot_of = [&](int i) { return i < c ? 2 * i + 1 : 2 * i; };
-    auto has = [&](int i) { return i < c ? s_kt0[c] > 0 : s_kt1[i] > s_kt0[i]; };
-    float m = -INFINITY;
-#pragma unroll 4
-    for (int i = c - 1; i <= end; ++i)
-      if (has(i)) m = fmaxf(m, p.part_ml[(size_t)slot_of(i) * 256 + row].x);
-    float b2 = -INFINITY;
-    if (p.o_more) {
-      b2 = p.lse_more[orow] * 1.4426950408889634f;
-      m = fmaxf(m, b2);
-    }
-    float l = 0.f, acc[8];
+    if ((w && item.y <= p.tok_tile) || lr >= p.tok_tile * p.group || tok >= item.y) continue;
+    const int64_t orow = (int64_t)(item.x + tok) * p.n_q_heads + item.z * p.group + (lr - tok_in * p.group);
+    // one pass with a running maximum, a batch of pieces at a time
+    float m = -INFINITY, l = 0.f, acc[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = 0.f;
-#pragma unroll 4
-    for (int i = c - 1; i <= end; ++i) {
-      if (!has(i)) continue;
-      const float2 ml = p.part_ml[(size_t)slot_of(i) * 256 + row];
-      const float4* po = p.part_o + (size_t)slot_of(i) * 32 * 256 + (size_t)col * 2 * 256 + row;
-      const float4 x = po[0], y = po[256];
-      const float f = ml.x == -INFINITY ? (ml.y == ml.y ? 0.f : ml.y) : exp2f(ml.x - m);
-      l += ml.y * f;
-      acc[0] += x.x * f; acc[1] += x.y * f; acc[2] += x.z * f; acc[3] += x.w * f;
-      acc[4] += y.x * f; acc[5] += y.y * f; acc[6] += y.z * f; acc[7] += y.w * f;
+    if (p.o_more) {
+      m = p.lse_more[orow] * 1.4426950408889634f;
+      if (m != -INFINITY) {
+        const float4* more = reinterpret_cast<const float4*>(p.o_more + orow * kHeadDim + col * 8);
+        const float4 x = more[0], y = more[1];
+        l = 1.f;
+        acc[0] = x.x; acc[1] = x.y; acc[2] = x.z; acc[3] = x.w; acc[4] = y.x; acc[5] = y.y; acc[6] = y.z; acc[7] = y.w;
+      }
     }
-    if (b2 != -INFINITY) {
-      const float f = exp2f(b2 - m);
-      l += f;
-      const float* more = p.o_more + orow * kHeadDim + col * 8;
+    for (int i0 = 0; i0 < n; i0 += kPjBatch) {
+      float2 ml[kPjBatch];
+      float4 x[kPjBatch], y[kPjBatch];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = fmaf(more[e], f, acc[e]);
+      for (int k = 0; k < kPjBatch; ++k) {
+        ml[k] = make_float2(-INFINITY, 0.f);
+        x[k] = y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i0 + k < n) {
+          const size_t slot = slots[i0 + k];
+          ml[k] = p.part_ml[slot * 256 + row];
+          const float4* po = p.part_o + slot * 32 * 256 + (size_t)col * 2 * 256 + row;
+          x[k] = po[0];
+          y[k] = po[256];
+        }
+      }
+      float mn = m;
+#pragma unroll
+      for (int k = 0; k < kPjBatch; ++k) mn = fmaxf(mn, ml[k].x);
+      const float keep = m == -INFINITY ? 0.f : fast_exp2(m - mn);
+      m = mn;
+      l *= keep;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] *= keep;
+#pragma unroll
+      for (int k = 0; k < kPjBatch; ++k) {
+        const float f = ml[k].x == -INFINITY ? (ml[k].y == ml[k].y ? 0.f : ml[k].y) : fast_exp2(ml[k].x - m);
+        l += ml[k].y * f;
+        acc[0] += x[k].x * f; acc[1] += x[k].y * f; acc[2] += x[k].z * f; acc[3] += x[k].w * f;
+        acc[4] += y[k].x * f; acc[5] += y[k].y * f; acc[6] += y[k].z * f; acc[7] += y[k].w * f;
+      }
     }
     const float inv = l > 0.f ? 1.f / l : (l != l ? l : 0.f);
 #pragma unroll

@@ -6,6 +6,7 @@ import os
 import random
 import re
 
+import numpy as np
 import pytest
 
 SRC = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "peerkv_b200", "csrc",
@@ -36,7 +37,15 @@ def items(seqs, hkv, group, causal):
 
 
 def cut(y, cost, n):
-    return 0 if y <= 0 else n if y >= cost else y * n // cost
+    """As the kernel rounds it: single precision (its quotient may differ in the last bits; what
+    has to hold is that all CTAs use the same ascending function)."""
+    if y <= 0 or n == 0:
+        return 0
+    return n if y >= cost else min(n, int(np.float32(y) * (np.float32(n) / np.float32(cost))))
+
+
+def piece(total, c, n_cta):
+    return total if c >= n_cta else int(float(total * c) * (1.0 / n_cta))
 
 
 def pieces(its, total, grid):
@@ -44,7 +53,7 @@ def pieces(its, total, grid):
     n_cta = min(grid, -(-total // MIN_PIECE))
     work, rec = [], []
     for c in range(n_cta):
-        x0, x1 = total * c // n_cta, total * (c + 1) // n_cta
+        x0, x1 = piece(total, c, n_cta), piece(total, c + 1, n_cta)
         assert x1 > x0
         mine, first = [], None
         for i, (a, cost, n, _) in enumerate(its):
