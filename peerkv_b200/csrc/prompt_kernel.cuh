@@ -52,8 +52,10 @@ constexpr int kPaMaxCtas = 256;
 constexpr int kPaSoftmaxRegs = 208;
 constexpr int kPaOtherRegs = 80;
 constexpr uint32_t kPaColO = 256;                        // TMEM columns: S0 0, S1 128, O0 256, O1 384
-constexpr int kPaItemCost = 384;   // what an item costs besides its keys, in keys
-constexpr int kPaMinPiece = 512;   // no CTA gets less than this many keys of work
+// The cost axis counts thirds of a step of 128 keys x 2 row tiles (3100 cycles).  A step with one row
+// tile takes two thirds of that, an item besides its steps as long as 3 of them.
+constexpr int kPaItemCost = 1152;  // per item, = 3 x 384 keys
+constexpr int kPaMinPiece = 1536;  // no CTA gets less, = 3 x 512 keys
 
 // Which CTA found which item cut (one per CTA, for the join).
 struct PromptRec {
@@ -93,7 +95,7 @@ struct PromptParams {
 struct PromptSeq {
   int q0, n, len, k0;          // packed first row, new tokens, cached tokens, first packed key
   int tiles;                   // items per kv-head
-  int64_t step, add;           // item t costs add + step * (t + 1)
+  int64_t step, add;           // item t costs add + step * (t + 1), in thirds of a key
 };
 
 __device__ __forceinline__ PromptSeq prompt_seq(const PromptParams& p, int s) {
@@ -110,8 +112,9 @@ __device__ __forceinline__ PromptSeq prompt_seq(const PromptParams& p, int s) {
   }
   const int tt = 2 * p.tok_tile;
   r.tiles = (r.n + tt - 1) / tt;
-  r.step = p.causal ? tt : 0;
-  r.add = (p.causal ? max(r.len - r.n, 0) : r.len) + kPaItemCost;
+  const int w = r.n > p.tok_tile ? 3 : 2;
+  r.step = p.causal ? w * tt : 0;
+  r.add = (int64_t)w * (p.causal ? max(r.len - r.n, 0) : r.len) + kPaItemCost;
   return r;
 }
 __device__ __forceinline__ int64_t prompt_items_cost(const PromptSeq& s, int64_t t) {   // of items 0 .. t-1
@@ -724,18 +727,20 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
               tma_load_4d_keep(dst + kPaHalfBytes, map, bar, 64, h, k0 + key0, 0);
             }
           } else {
+            int pg[8];                                     // at most 128 / 16 boxes of a half tile
+#pragma unroll
+            for (int b = 0; b < 8; ++b) pg[b] = __shfl_sync(0xffffffffu, page, b);
             int tok = key0 % p.page_size;
-#pragma unroll 1
-            for (int b = 0; b < n_box; ++b) {
-              const int pg = uniform(__shfl_sync(0xffffffffu, page, b));
-              const int c1 = p.head_major ? tok : h, c2 = p.head_major ? h : tok;
-              if (elect_one()) {
-                tma_load_4d_keep(dst + b * box_bytes, map, bar, 0, c1, c2, pg);
-                tma_load_4d_keep(dst + kPaHalfBytes + b * box_bytes, map, bar, 64, c1, c2, pg);
+            if (elect_one()) {
+#pragma unroll
+              for (int b = 0; b < 8; ++b) {
+                if (b >= n_box) break;
+                const int c1 = p.head_major ? tok : h, c2 = p.head_major ? h : tok;
+                tma_load_4d_keep(dst + b * box_bytes, map, bar, 0, c1, c2, pg[b]);
+                tma_load_4d_keep(dst + kPaHalfBytes + b * box_bytes, map, bar, 64, c1, c2, pg[b]);
+                tok += p.box_tok;
+                if (tok >= p.page_size) tok = 0;
               }
-              __syncwarp();
-              tok += p.box_tok;
-              if (tok >= p.page_size) tok = 0;
             }
           }
           __syncwarp();

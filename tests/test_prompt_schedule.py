@@ -28,7 +28,8 @@ def items(seqs, hkv, group, causal):
         tiles = -(-n // tt)
         for _ in range(hkv):
             for t in range(tiles):
-                cost = (max(length - n, 0) if causal else length) + ITEM_COST + (tt * (t + 1) if causal else 0)
+                w = 3 if n > tt // 2 else 2
+                cost = w * (max(length - n, 0) if causal else length) + ITEM_COST + (w * tt * (t + 1) if causal else 0)
                 n_tok = min(tt, n - t * tt)
                 vis = max(0, min(length, length - n + t * tt + n_tok)) if causal else length
                 out.append((a, cost, -(-vis // KEYS), n_tok))
