@@ -1515,12 +1515,27 @@ extern "C" int pkv_norm_rope_append(int device, const pkv_append_args* a, uint32
   }
   DeviceGuard guard(device);
   if (!guard.ok) return fail(PKV_E_CUDA, "cannot select device %d", device);
-  const int rows = p.n_q_heads + (p.slot_mapping ? 2 * p.n_kv_heads : 0);
-  const dim3 grid(p.n_tokens, (rows + pkv::kNraRows - 1) / pkv::kNraRows);
+  // A warp per token once that is 16 warps per SM (the angles are then made once per token); below that
+  // its rows are split, down to one pair per warp.
+  int splits = (p.n_q_heads + 1) / 2 + (p.slot_mapping ? 2 * ((p.n_kv_heads + 1) / 2) : 0);
+  while (splits > 1 && (int64_t)p.n_tokens * (splits / 2) >= 2368) splits = (splits + 1) / 2;
+  const int64_t blocks = ((int64_t)p.n_tokens * splits + pkv::kNraWarps - 1) / pkv::kNraWarps;
+  if (blocks > 0x7fffffff) return fail(PKV_E_UNSUPPORTED, "n_tokens %d", p.n_tokens);
+  const unsigned int grid = (unsigned int)blocks;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   Range range("pkv:norm_rope_append");
-  if (a->dtype == PKV_BF16) pkv::norm_rope_append_kernel<true><<<grid, pkv::kNraThreads, 0, st>>>(p);
-  else                      pkv::norm_rope_append_kernel<false><<<grid, pkv::kNraThreads, 0, st>>>(p);
+  auto launch = [&](auto kernel) { kernel<<<grid, pkv::kNraWarps * 32, 0, st>>>(p, splits); };
+  const bool quant = p.slot_mapping && is_quant(p.fmt);
+  switch ((a->dtype == PKV_BF16 ? 4 : 0) | (p.interleaved ? 2 : 0) | (quant ? 1 : 0)) {
+    case 0: launch(pkv::norm_rope_append_kernel<false, false, false>); break;
+    case 1: launch(pkv::norm_rope_append_kernel<false, false, true>); break;
+    case 2: launch(pkv::norm_rope_append_kernel<false, true, false>); break;
+    case 3: launch(pkv::norm_rope_append_kernel<false, true, true>); break;
+    case 4: launch(pkv::norm_rope_append_kernel<true, false, false>); break;
+    case 5: launch(pkv::norm_rope_append_kernel<true, false, true>); break;
+    case 6: launch(pkv::norm_rope_append_kernel<true, true, false>); break;
+    default: launch(pkv::norm_rope_append_kernel<true, true, true>); break;
+  }
   PKV_CUDA(cudaGetLastError());
   return PKV_OK;
 }
