@@ -19,6 +19,12 @@ Per layer, on the home GPU (everything but attention lives there, as in the refe
 and one `pkv_peer_step` per layer on every peer.  New tokens are appended to pages that
 the home GPU owns ("newest page local"), so the append is a local write.
 
+Models that norm q and k per head, turn a part of a head or interleaved pairs
+(`LlamaGeometry.qk_norm`, `rotary_dim`, `rope_interleaved`) go through
+`ops.norm_rope_append` instead of pkv_rope_append.  On one GPU, `PromptStep` runs packed
+prompts (or chunks of them) through the same layers and fills the cache, and a `DecodeStep`
+whose sequences share prefixes (`prefix=`) reads each prefix once per group.
+
 `capture()` records the WHOLE step of a rank -- all layers, attention launches included --
 as one CUDA graph per GPU (the reference captures its two-device step the same way,
 csrc/peer_rt_bench.cu:134-154, csrc/peer_fused_decoder.cu:433-455).  The attention kernels
@@ -35,7 +41,7 @@ from typing import List, Optional
 import torch
 
 from . import _lib, ops
-from ._lib import check
+from ._lib import PeerKVError, check
 
 
 @dataclass
@@ -49,6 +55,14 @@ class LlamaGeometry:
     vocab: int = 128256
     rms_eps: float = 1e-5
     rope_theta: float = 500000.0
+    qk_norm: bool = False               # RMS norm of every q and k head before the rotation
+    rotary_dim: Optional[int] = None    # how much of a head turns (None: all of it)
+    rope_interleaved: bool = False      # neighbours turn against each other instead of halves
+
+    @property
+    def plain_rope(self) -> bool:
+        """What pkv_rope_append covers."""
+        return not self.qk_norm and not self.rope_interleaved and self.rotary_dim in (None, self.head_dim)
 
 
 class LayerWeights:
@@ -62,6 +76,8 @@ class LayerWeights:
         self.w_down = w(g.ffn, g.hidden)
         self.norm1 = torch.ones(g.hidden, dtype=dtype, device=device)
         self.norm2 = torch.ones(g.hidden, dtype=dtype, device=device)
+        self.q_norm = torch.ones(g.head_dim, dtype=dtype, device=device) if g.qk_norm else None
+        self.k_norm = torch.ones(g.head_dim, dtype=dtype, device=device) if g.qk_norm else None
 
 
 class ModelWeights:
@@ -77,7 +93,8 @@ class ModelWeights:
     def bytes(self) -> int:
         n = self.embed.numel() + self.lm_head.numel() + self.final_norm.numel()
         for l in self.layers:
-            n += sum(t.numel() for t in (l.wqkv, l.wo, l.w_gate_up, l.w_down, l.norm1, l.norm2))
+            n += sum(t.numel() for t in (l.wqkv, l.wo, l.w_gate_up, l.w_down, l.norm1, l.norm2, l.q_norm, l.k_norm)
+                     if t is not None)
         return n * self.embed.element_size()
 
 
@@ -150,14 +167,20 @@ class DecodeStep:
     distributed.DistPeerGroup) or, with no group, through a one-GPU shard.  Peer rank
     (weights None): one peer step per layer.  `append_slots` = (page ids [B], token slots
     [B]) int64 on the home GPU: where each sequence's new token goes in every layer's pool.
+    `prefix` (one GPU only) = (prefix_table, prefix_lens, group_offsets) as in
+    ops.decode_shared_prefix; the layers' tables and lengths then describe what each sequence
+    has behind its group's prefix.
     """
 
     def __init__(self, g: LlamaGeometry, weights: Optional[ModelWeights], kv: List[ShardedKVLayer], batch: int,
-                 device, group=None, append_slots=None):
+                 device, group=None, append_slots=None, prefix=None):
         self.g, self.w, self.kv, self.group = g, weights, kv, group
         self.dev = torch.device(device)
         self.B = batch
         self.append_slots = append_slots
+        self.prefix = prefix
+        if prefix is not None and group is not None:
+            raise PeerKVError("a shared prefix lives on one GPU: it cannot be combined with a group")
         self.scale = 1.0 / math.sqrt(g.head_dim)
         self._graph = None
         dev, dt = self.dev, torch.bfloat16 if weights is None else weights.embed.dtype
@@ -175,12 +198,16 @@ class DecodeStep:
             self.gu, self.act = z(batch, 2 * g.ffn), z(batch, g.ffn)
             self.logits = z(batch, g.vocab)
             self.next = z(batch, d=torch.int64)
-            self.inv_freq = rope_inv_freq(g.head_dim, g.rope_theta, dev)
+            self.inv_freq = rope_inv_freq(g.rotary_dim or g.head_dim, g.rope_theta, dev)
 
     # -- attention of one layer ---------------------------------------------------------- #
     def _attend(self, li: int):
         L, st = _lib.lib(), ops._stream(self.dev)
-        if self.group is None:
+        if self.prefix is not None:
+            l, (pt, pl, go) = self.kv[li], self.prefix
+            ops.decode_shared_prefix(self.q, l.pool[0], l.pool[1], pt, pl, l.table, l.lens, group_offsets=go,
+                                     scale=self.scale, out=self.ao, shard=self.shard)
+        elif self.group is None:
             check(L.pkv_decode(self.shard._h, C.byref(self.args[li]), self.ao.data_ptr(), ops._DT[self.ao.dtype],
                                None, st))
         else:
@@ -200,7 +227,13 @@ class DecodeStep:
             torch.matmul(self.h, lw.wqkv, out=self.qkv)
             pool = self.kv[li].pool if self.append_slots is not None else None
             pages, slots = self.append_slots if self.append_slots is not None else (None, None)
-            rope_append(self.qkv, self.pos, self.inv_freq, self.q, g.n_q_heads, g.n_kv_heads, pool, pages, slots)
+            if g.plain_rope:
+                rope_append(self.qkv, self.pos, self.inv_freq, self.q, g.n_q_heads, g.n_kv_heads, pool, pages, slots)
+            else:
+                k, v, slot = (None, None, None) if pool is None else (pool[0], pool[1], pages * pool.shape[2] + slots)
+                ops.norm_rope_append(self.qkv, self.pos, self.inv_freq, g.n_q_heads, g.n_kv_heads, self.q, k, v, slot,
+                                     q_weight=lw.q_norm, k_weight=lw.k_norm, eps=g.rms_eps,
+                                     interleaved=g.rope_interleaved)
             self._attend(li)
             torch.matmul(self.ao.view(self.B, -1), lw.wo, out=self.proj)
             add_rmsnorm(self.x, self.proj, lw.norm2, self.h, g.rms_eps)
@@ -259,3 +292,39 @@ class DecodeStep:
                 self.group.step(self.args[li])
             else:
                 self._attend(li)
+
+
+class PromptStep:
+    """Prompts through the model on one GPU: packed sequences of different lengths, whole or as the
+    next chunk behind what the cache holds already.  Fills every layer's pages and returns the
+    logits of each sequence's last token."""
+
+    def __init__(self, g: LlamaGeometry, weights: ModelWeights, kv: List[ShardedKVLayer], device):
+        self.g, self.w, self.kv = g, weights, kv
+        self.dev = torch.device(device)
+        self.inv_freq = rope_inv_freq(g.rotary_dim or g.head_dim, g.rope_theta, self.dev)
+
+    def step(self, tokens: torch.Tensor, positions: torch.Tensor, slot_mapping: torch.Tensor,
+             cu_seqlens: torch.Tensor, seq_lens: torch.Tensor) -> torch.Tensor:
+        """tokens, positions, slot_mapping [T] int64 (page * page size + offset of this GPU's pools);
+        cu_seqlens [n + 1] int32 offsets of the sequences in them; seq_lens [n] int32 tokens of
+        each in the cache, the new ones included -> logits [n, vocab]."""
+        g, T = self.g, tokens.shape[0]
+        dt = self.w.embed.dtype
+        x = self.w.embed.index_select(0, tokens)
+        h = torch.empty_like(x)
+        act = torch.empty(T, g.ffn, dtype=dt, device=self.dev)
+        delta = None
+        for l, lw in zip(self.kv, self.w.layers):
+            add_rmsnorm(x, delta, lw.norm1, h, g.rms_eps)
+            qkv = torch.matmul(h, lw.wqkv)
+            q = qkv[:, :g.n_q_heads * g.head_dim].view(T, g.n_q_heads, g.head_dim)     # turned where it lies
+            ops.norm_rope_append(qkv, positions, self.inv_freq, g.n_q_heads, g.n_kv_heads, q, l.pool[0], l.pool[1],
+                                 slot_mapping, q_weight=lw.q_norm, k_weight=lw.k_norm, eps=g.rms_eps,
+                                 interleaved=g.rope_interleaved)
+            ao = ops.prefill_paged(q, l.pool[0], l.pool[1], l.table, seq_lens, cu_seqlens)
+            add_rmsnorm(x, torch.matmul(ao.view(T, -1), lw.wo), lw.norm2, h, g.rms_eps)
+            swiglu(torch.matmul(h, lw.w_gate_up), act)
+            delta = torch.matmul(act, lw.w_down)
+        add_rmsnorm(x, delta, self.w.final_norm, h, g.rms_eps)
+        return torch.matmul(h.index_select(0, cu_seqlens[1:].long() - 1), self.w.lm_head)

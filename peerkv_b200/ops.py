@@ -21,7 +21,8 @@ HEAD_DIM = 128
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """Handle of torch's current stream on the device (without the Stream object, which costs 2 us)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 
 def _require_cuda(t: torch.Tensor, name: str):
@@ -134,14 +135,11 @@ def paged_view(k_pool: torch.Tensor, v_pool: torch.Tensor,
         raise PeerKVError("the head dimension must be contiguous")
     if k_pool.dtype not in _DT or k_pool.dtype == torch.float32:
         raise PeerKVError(f"unsupported KV dtype {k_pool.dtype}")
-    v = KvView()
-    v.k, v.v = k_pool.data_ptr(), v_pool.data_ptr()
-    v.k_scale = k_scale.data_ptr() if k_scale is not None else None
-    v.v_scale = v_scale.data_ptr() if v_scale is not None else None
-    v.dtype = _DT[k_pool.dtype]
-    v.n_pages, v.page_size, v.n_kv_heads, v.head_dim = k_pool.shape
-    v.page_stride, v.token_stride, v.head_stride = k_pool.stride(0), k_pool.stride(1), k_pool.stride(2)
-    return v
+    n_pages, page_size, n_kv_heads, head_dim = k_pool.shape
+    st = k_pool.stride()
+    return KvView(k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr() if k_scale is not None else None,
+                  v_scale.data_ptr() if v_scale is not None else None, _DT[k_pool.dtype], n_kv_heads, head_dim,
+                  page_size, n_pages, st[0], st[1], st[2])
 
 
 def contiguous_view(K: torch.Tensor, V: torch.Tensor) -> KvView:
@@ -338,8 +336,10 @@ def _rows_of_heads(t: torch.Tensor, name: str) -> torch.Tensor:
     multiples of 8 elements, 16-byte aligned; anything else is copied."""
     if t.dim() != 3 or t.shape[2] != HEAD_DIM:
         raise PeerKVError(f"{name} must be [tokens, heads, {HEAD_DIM}]; got {tuple(t.shape)}")
-    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and \
-        all(n <= 1 or (st > 0 and st % 8 == 0) for n, st in zip(t.shape[:2], t.stride()[:2]))
+    n0, n1, _ = t.shape
+    s0, s1, s2 = t.stride()
+    ok = s2 == 1 and t.data_ptr() % 16 == 0 and (n0 <= 1 or (s0 > 0 and s0 % 8 == 0)) and \
+        (n1 <= 1 or (s1 > 0 and s1 % 8 == 0))
     return t if ok or t.numel() == 0 else t.contiguous()
 
 
@@ -362,24 +362,20 @@ def _check_out(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
 
 def _prompt_call(q, view, scale, causal, out, lse, cu_q, n_seqs, status, block_table=None, seq_lens=None, cu_k=None,
                  more=None):
-    a = _lib.PromptArgs()
-    a.q, a.q_token_stride, a.q_head_stride = q.data_ptr(), q.stride(0), q.stride(1)
-    a.dtype, a.n_q_heads, a.total_q, a.n_seqs = _DT[q.dtype], q.shape[1], q.shape[0], n_seqs
-    a.cu_seqlens_q = cu_q.data_ptr()
-    a.kv = view
-    if block_table is not None:
-        a.block_table, a.block_table_stride, a.block_table_cols = \
-            block_table.data_ptr(), block_table.stride(0), block_table.shape[1]
-        a.seq_lens = seq_lens.data_ptr()
-    else:
-        a.cu_seqlens_k = cu_k.data_ptr()
-    if more is not None:
-        a.o_more, a.lse_more = more[0].data_ptr(), more[1].data_ptr()
-    a.scale, a.causal = float(scale), 1 if causal else 0
-    ws = _prompt_workspace(q.device)
-    check(_lib.lib().pkv_prompt_attention(q.device.index, C.byref(a), out.data_ptr(), _DT[out.dtype],
+    dev = q.device
+    total_q, n_heads, _ = q.shape
+    st = q.stride()
+    paged = block_table is not None
+    a = _lib.PromptArgs(q.data_ptr(), st[0], st[1], _DT[q.dtype], n_heads, total_q, n_seqs, cu_q.data_ptr(), view,
+                        block_table.data_ptr() if paged else None, block_table.stride(0) if paged else 0,
+                        block_table.shape[1] if paged else 0, 1 if causal else 0,
+                        seq_lens.data_ptr() if paged else None, None if paged else cu_k.data_ptr(),
+                        more[0].data_ptr() if more is not None else None,
+                        more[1].data_ptr() if more is not None else None, scale, 0)
+    ws = _prompt_workspace(dev)
+    check(_lib.lib().pkv_prompt_attention(dev.index, C.byref(a), out.data_ptr(), _DT[out.dtype],
                                           lse.data_ptr() if lse is not None else None, ws.data_ptr(), ws.numel(),
-                                          _status_word(status, q.device), _stream(q.device)))
+                                          _status_word(status, dev), _stream(dev)))
 
 
 def _check_prompt_q(q: torch.Tensor) -> torch.Tensor:
@@ -463,11 +459,9 @@ def prefill_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens
     ck = cu if cu_seqlens_k is None else _cu(cu_seqlens_k, q.device, "cu_seqlens_k")
     if ck.numel() != cu.numel():
         raise PeerKVError("cu_seqlens_q and cu_seqlens_k must describe the same number of sequences")
-    view = KvView()
-    view.k, view.v = k.data_ptr(), v.data_ptr()
-    view.dtype, view.n_kv_heads, view.head_dim = _DT[k.dtype], k.shape[1], HEAD_DIM
-    view.page_size, view.n_pages = k.shape[0], 1 if k.shape[0] > 0 else 0
-    view.token_stride, view.head_stride, view.page_stride = k.stride(0), k.stride(1), HEAD_DIM
+    total_k, n_kv, _ = k.shape
+    view = KvView(k.data_ptr(), v.data_ptr(), None, None, _DT[k.dtype], n_kv, HEAD_DIM, total_k, 1 if total_k > 0 else 0,
+                  HEAD_DIM, k.stride(0), k.stride(1))
     out = _check_out(out, q)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
     _prompt_call(q, view, 1.0 / math.sqrt(HEAD_DIM) if scale is None else scale, causal, out, lse, cu, cu.numel() - 1,
@@ -513,6 +507,12 @@ def decode_shared_prefix(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     return (out, lse) if return_lse else out
 
 
+def _vector(t: torch.Tensor, n: int, dt, device, name: str) -> torch.Tensor:
+    if t.dtype != dt or t.device != device or t.dim() != 1 or t.numel() != n:
+        raise PeerKVError(f"{name} must be {dt} [{n}] on {device}; got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
 def norm_rope_append(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optional[torch.Tensor], n_q_heads: int,
                      n_kv_heads: int, q_out: Optional[torch.Tensor] = None, k_pool: Optional[torch.Tensor] = None,
                      v_pool: Optional[torch.Tensor] = None, slot_mapping: Optional[torch.Tensor] = None, k_scale=None,
@@ -546,54 +546,50 @@ def norm_rope_append(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optio
             (T and (q_out.stride(2) != 1 or (n_q_heads > 1 and q_out.stride(1) != HEAD_DIM))):
         raise PeerKVError(f"q_out must be [T, n_q_heads, {HEAD_DIM}] of qkv's dtype and GPU with contiguous heads")
 
-    def vector(t, n, dt, name):
-        if t is None:
-            return None
-        if t.device != dev or t.dtype != dt or t.dim() != 1 or t.numel() != n:
-            raise PeerKVError(f"{name} must be {dt} [{n}] on {dev}; got {t.dtype} {tuple(t.shape)} on {t.device}")
-        return t if t.is_contiguous() else t.contiguous()
-
     half = 0 if inv_freq is None else inv_freq.numel()
-    pos = positions if positions.dtype == torch.int64 else positions.to(torch.int64)
-    keep = [qkv, vector(pos, T, torch.int64, "positions"), vector(inv_freq, half, torch.float32, "inv_freq"),
-            vector(q_weight, HEAD_DIM, qkv.dtype, "q_weight"), vector(k_weight, HEAD_DIM, qkv.dtype, "k_weight")]
-    a = _lib.AppendArgs()
-    a.qkv, a.qkv_stride = qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1]
-    a.positions, a.inv_freq, a.q_weight, a.k_weight = [t.data_ptr() if t is not None else None for t in keep[1:]]
-    a.q_out, a.q_out_stride = q_out.data_ptr(), q_out.stride(0) if T > 1 else n_q_heads * HEAD_DIM
-    a.n_tokens, a.n_q_heads, a.n_kv_heads, a.head_dim = T, n_q_heads, n_kv_heads, HEAD_DIM
-    a.dtype, a.rot_dim, a.interleaved = _DT[qkv.dtype], 2 * half, 1 if interleaved else 0
-    a.eps, a.gain = float(eps), float(gain)
+    positions = _vector(positions if positions.dtype == torch.int64 else positions.to(torch.int64), T, torch.int64, dev,
+                        "positions")
+    if inv_freq is not None:
+        inv_freq = _vector(inv_freq, half, torch.float32, dev, "inv_freq")
+    if q_weight is not None:
+        q_weight = _vector(q_weight, HEAD_DIM, qkv.dtype, dev, "q_weight")
+    if k_weight is not None:
+        k_weight = _vector(k_weight, HEAD_DIM, qkv.dtype, dev, "k_weight")
+    views = first = None
+    n_dev = 0
     if slot_mapping is not None:
         if k_pool is None or v_pool is None:
             raise PeerKVError("an append needs k_pool, v_pool and slot_mapping")
-        sm = slot_mapping if slot_mapping.dtype == torch.int64 else slot_mapping.to(torch.int64)
-        keep.append(vector(sm, T, torch.int64, "slot_mapping"))
-        a.slot_mapping = keep[-1].data_ptr()
+        slot_mapping = _vector(slot_mapping if slot_mapping.dtype == torch.int64 else slot_mapping.to(torch.int64), T,
+                               torch.int64, dev, "slot_mapping")
         pools = [(k_pool, v_pool, k_scale, v_scale)] + [tuple(p) + (None,) * (4 - len(p)) for p in peers]
-        if len(bases) != len(pools) - 1:
+        n_dev = len(pools)
+        if len(bases) != n_dev - 1:
             raise PeerKVError("every peer pool needs its first page id in bases")
         _same_gpu(k_pool, dev, "k_pool")
-        views = (KvView * len(pools))()
+        views = (KvView * n_dev)()
         for i, (kp, vp, ks, vs) in enumerate(pools):
-            for t in (vp, ks, vs):
-                _same_gpu(t, kp.device, f"pool {i}")
-            if kp.dtype != vp.dtype or kp.dtype not in (qkv.dtype, torch.int8, torch.float8_e4m3fn):
-                raise PeerKVError(f"pool {i}: {kp.dtype} / {vp.dtype}; qkv's dtype, int8 or float8_e4m3fn")
-            if kp.element_size() == 1:
+            _same_gpu(vp, kp.device, "v_pool"); _same_gpu(ks, kp.device, "k_scale"); _same_gpu(vs, kp.device, "v_scale")
+            kdt = kp.dtype
+            if kdt != vp.dtype or (kdt != qkv.dtype and kdt not in (torch.int8, torch.float8_e4m3fn)):
+                raise PeerKVError(f"pool {i}: {kdt} / {vp.dtype}; qkv's dtype, int8 or float8_e4m3fn")
+            if kdt != qkv.dtype:
                 for t in (ks, vs):
                     if t is None or t.dtype != torch.float16 or t.shape != kp.shape[:3] or not t.is_contiguous():
                         raise PeerKVError("quantised pools need contiguous fp16 k_scale / v_scale [n_pages, page, Hkv]")
-            if kp.shape[2] != n_kv_heads or kp.shape[3] != HEAD_DIM:
+            if kp.dim() != 4 or kp.shape[2] != n_kv_heads or kp.shape[3] != HEAD_DIM:
                 raise PeerKVError(f"pool {i} must be [n_pages, page, {n_kv_heads}, {HEAD_DIM}]; got {tuple(kp.shape)}")
             views[i] = paged_view(kp, vp, ks, vs)
         if peers:
             from .peerkv.kv_alloc import _enable_peer_access
             _enable_peer_access(dev, [p[0].device for p in pools[1:]])
-        a.pools, a.n_dev = views, len(pools)
-        first = (C.c_int64 * len(pools))(0, *[int(b) for b in bases])
-        a.bases = first
+        first = (C.c_int64 * n_dev)(0, *[int(b) for b in bases])
     elif k_pool is not None or v_pool is not None:
         raise PeerKVError("an append needs k_pool, v_pool and slot_mapping")
+    ptr = lambda t: t.data_ptr() if t is not None else None
+    a = _lib.AppendArgs(qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1], positions.data_ptr(), ptr(inv_freq),
+                        ptr(q_weight), ptr(k_weight), q_out.data_ptr(),
+                        q_out.stride(0) if T > 1 else n_q_heads * HEAD_DIM, ptr(slot_mapping), views, first, n_dev, T,
+                        n_q_heads, n_kv_heads, HEAD_DIM, _DT[qkv.dtype], 2 * half, 1 if interleaved else 0, eps, gain)
     check(_lib.lib().pkv_norm_rope_append(dev.index, C.byref(a), _status_word(status, dev), _stream(dev)))
     return q_out
