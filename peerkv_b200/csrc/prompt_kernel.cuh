@@ -121,10 +121,12 @@ __device__ __forceinline__ int64_t prompt_items_cost(const PromptSeq& s, int64_t
   return t * s.add + s.step * (t * (t + 1) / 2);
 }
 
-// Where CTA c's piece of the cost axis starts.  All CTAs compute it alike, so it may be rounded as it
-// likes as long as it ascends; a 64-bit integer division costs some 300 cycles of the start.
-__device__ __forceinline__ int64_t prompt_cut(int64_t total, int c, int n_cta, double inv) {
-  return c >= n_cta ? total : (int64_t)((double)(total * c) * inv);
+// Length of a CTA's piece of the cost axis: total / n_cta, a little more where the single-precision
+// quotient needs it so that n_cta pieces cover the axis.  No piece is empty: one is at least 768
+// long (kPaMinPiece), and what it is too long by, times n_cta, stays below that.  (A 64-bit or
+// double-precision division costs the start of every CTA some hundred cycles.)
+__device__ __forceinline__ int64_t prompt_piece(int64_t total, int n_cta) {
+  return (int64_t)((float)total * __fdividef(1.f, (float)n_cta)) + (total >> 20) + 1;
 }
 
 struct PromptItem {
@@ -153,7 +155,7 @@ struct PromptItem {
   // first item of the piece (fill() follows): s, seq and `base`, the cost before s, are known
   __device__ __forceinline__ void start(const PromptParams& p, int64_t base) {
     const int64_t per = prompt_items_cost(seq, seq.tiles);
-    h = (int)((float)(x0 - base) / (float)per);          // about; the next lines make it exact
+    h = (int)__fdividef((float)(x0 - base), (float)per);  // about; the next lines make it exact
     h = min(max(h, 0), p.n_kv_heads - 1);
     while (h > 0 && h * per > x0 - base) --h;
     while (h + 1 < p.n_kv_heads && (h + 1) * per <= x0 - base) ++h;
@@ -333,9 +335,8 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   }
   const int n_cta = (int)min((int64_t)gridDim.x, (total + kPaMinPiece - 1) / kPaMinPiece);
   const bool active = (int)blockIdx.x < n_cta;
-  const double inv = active ? 1.0 / n_cta : 0.0;
-  const int64_t x0 = active ? prompt_cut(total, blockIdx.x, n_cta, inv) : 0;
-  const int64_t x1 = active ? prompt_cut(total, blockIdx.x + 1, n_cta, inv) : 0;
+  const int64_t piece = active ? prompt_piece(total, n_cta) : 0;
+  const int64_t x0 = blockIdx.x * piece, x1 = min(total, x0 + piece);
   if (active && before <= x0 && x0 < before + mine) {
     int64_t base = before;
     for (int s = sb; s < se; ++s) {
@@ -685,22 +686,6 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       while (ok && (kv == 0 ? make() : take())) {
         const int n_tiles = uniform(wk.n_tiles), h = uniform(wk.h), two = uniform(wk.two);
         if (n_tiles == 0) continue;
-        // Q: the group's heads of up to 2 * tok_tile tokens, in two halves of 64 values
-        if (kv == 0) {
-          if (!(ok = pa_wait(q_empty, (n_q & 1) ^ 1, abort_flag))) break;
-          ++n_q;
-          const int q0 = uniform(wk.q0);
-          if (elect_one()) {
-            const uint32_t half = (uint32_t)p.tok_tile * p.group * 128u;
-            mbar_arrive_expect_tx(q_full, half * (two ? 4u : 2u));
-#pragma unroll 1
-            for (int w = 0; w < (two ? 2 : 1); ++w)
-              for (int d = 0; d < 2; ++d)
-                tma_load_3d(smem + w * kPaTileBytes + d * kPaHalfBytes, &qmap, q_full, d * 64, h * p.group,
-                            q0 + w * p.tok_tile);
-          }
-          __syncwarp();
-        }
         const int kt0 = uniform(wk.kt0), vis = uniform(wk.vis), k0 = uniform(wk.k0);
         const int32_t* row = paged ? p.block_table + (int64_t)wk.s * p.bt_stride : nullptr;
         // lane b: the page of box b of tile i, read a few tiles ahead of its use
@@ -747,6 +732,22 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           return true;
         };
         int p0 = fetch(0), p1 = fetch(1), p2 = fetch(2);
+        // Q: the group's heads of up to 2 * tok_tile tokens, in two halves of 64 values
+        if (kv == 0) {
+          if (!(ok = pa_wait(q_empty, (n_q & 1) ^ 1, abort_flag))) break;
+          ++n_q;
+          const int q0 = uniform(wk.q0);
+          if (elect_one()) {
+            const uint32_t half = (uint32_t)p.tok_tile * p.group * 128u;
+            mbar_arrive_expect_tx(q_full, half * (two ? 4u : 2u));
+#pragma unroll 1
+            for (int w = 0; w < (two ? 2 : 1); ++w)
+              for (int d = 0; d < 2; ++d)
+                tma_load_3d(smem + w * kPaTileBytes + d * kPaHalfBytes, &qmap, q_full, d * 64, h * p.group,
+                            q0 + w * p.tok_tile);
+          }
+          __syncwarp();
+        }
 #pragma unroll 1
         for (int i = 0; i < n_tiles && ok; ++i) {
           ok = load(i, p0);

@@ -45,16 +45,21 @@ def cut(y, cost, n):
     return n if y >= cost else min(n, int(np.float32(y) * (np.float32(n) / np.float32(cost))))
 
 
-def piece(total, c, n_cta):
-    return total if c >= n_cta else int(float(total * c) * (1.0 / n_cta))
+def piece(total, n_cta):
+    """As the kernel rounds it, with the quotient taken 2 steps of fp32 too low or too high (the bound
+    of its approximate division)."""
+    q = np.float32(total) * (np.float32(1.0) / np.float32(n_cta))
+    return [int(q * np.float32(1 + e * 2.0 ** -22)) + (total >> 20) + 1 for e in (-1, 0, 1)]
 
 
-def pieces(its, total, grid):
+def pieces(its, total, grid, which):
     """Per CTA: list of (item index, kt0, kt1, slot or None when written directly), and its record."""
     n_cta = min(grid, -(-total // MIN_PIECE))
+    size = piece(total, n_cta)[which]
+    assert size * n_cta >= total
     work, rec = [], []
     for c in range(n_cta):
-        x0, x1 = piece(total, c, n_cta), piece(total, c + 1, n_cta)
+        x0, x1 = c * size, min(total, c * size + size)
         assert x1 > x0
         mine, first = [], None
         for i, (a, cost, n, _) in enumerate(its):
@@ -92,7 +97,11 @@ def check(seqs, hkv, group, causal, grid):
     its, total = items(seqs, hkv, group, causal)
     if total == 0:
         return
-    work, rec = pieces(its, total, grid)
+    for which in range(3):
+        check_split(its, *pieces(its, total, grid, which))
+
+
+def check_split(its, work, rec):
     done = {i: [] for i in range(len(its))}
     written = {}
     for c, mine in enumerate(work):
@@ -126,6 +135,15 @@ def test_every_tile_once(seed):
         n = rng.choice([0, 1, 1, 2, 63, 64, 65, rng.randint(1, 3000)])
         seqs.append((n, rng.choice([0, n, n // 2, n + rng.randint(0, 20000)])))
     check(seqs, rng.choice([1, 2, 8]), rng.choice([1, 3, 4, 8, 128]), rng.random() < 0.6, rng.choice([1, 7, 148]))
+
+
+def test_pieces_cover_the_axis():
+    rng = random.Random(1)
+    for n_cta in list(range(1, 150)) + [256]:
+        for total in [1, 768 * n_cta + 1, MIN_PIECE * n_cta - 5] + [int(MIN_PIECE * n_cta * 10 ** rng.uniform(0, 8)) for _ in range(20)]:
+            n = min(n_cta, -(-total // MIN_PIECE))
+            for size in piece(total, n):
+                assert size * n >= total > size * (n - 1)
 
 
 def test_edge_lengths():
