@@ -708,8 +708,9 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
           __syncwarp();
           if (!paged) {
             if (elect_one()) {
-              tma_load_4d_keep(dst, map, bar, 0, h, k0 + key0, 0);
-              tma_load_4d_keep(dst + kPaHalfBytes, map, bar, 64, h, k0 + key0, 0);
+              const int c1 = p.head_major ? k0 + key0 : h, c2 = p.head_major ? h : k0 + key0;
+              tma_load_4d_keep(dst, map, bar, 0, c1, c2, 0);
+              tma_load_4d_keep(dst + kPaHalfBytes, map, bar, 64, c1, c2, 0);
             }
           } else {
             int pg[8];                                     // at most 128 / 16 boxes of a half tile

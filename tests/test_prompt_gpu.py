@@ -112,10 +112,12 @@ def test_strided_inputs_and_head_major_pools(dev):
 
 
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
-def test_packed_keys(dev, dt):
+@pytest.mark.parametrize("hq,hkv,lens", [
+    (8, 2, [1, 17, 0, 130, 64, 300]), (4, 1, [200, 3, 129]), (4, 4, [5, 260]),
+    (8, 4, [1]), (2, 1, [1]), (5, 1, [1, 1, 40])])       # strides of a dimension of one are anything
+def test_packed_keys(dev, dt, hq, hkv, lens):
     from peerkv_b200 import ops
     gen = torch.Generator().manual_seed(31)
-    hq, hkv, lens = 8, 2, [1, 17, 0, 130, 64, 300]
     total = sum(lens)
     qkv = torch.randn(total, (hq + 2 * hkv) * D, generator=gen).to(dt)
     heads = qkv.view(total, hq + 2 * hkv, D)
@@ -126,8 +128,13 @@ def test_packed_keys(dev, dt):
         parts.append(attend64(x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:], 1 / math.sqrt(D), 1 + torch.arange(n)))
     ref = [torch.cat(x) for x in zip(*parts)]
     g = qkv.to(dev).view(total, hq + 2 * hkv, D)
-    out, lse = ops.prefill_packed(g[:, :hq], g[:, hq:hq + hkv], g[:, hq + hkv:], cu.to(dev), return_lse=True)
+    q, k, v = g[:, :hq], g[:, hq:hq + hkv], g[:, hq + hkv:]
+    out, lse = ops.prefill_packed(q, k, v, cu.to(dev), return_lse=True)
     assert_close(out, lse, *ref, dt, max(lens))
+    # the same values laid out on their own, and head by head
+    assert torch.equal(ops.prefill_packed(q.contiguous(), k.contiguous(), v.contiguous(), cu.to(dev)), out)
+    by_head = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(ops.prefill_packed(by_head(q), by_head(k), by_head(v), cu.to(dev)), out)
 
 
 def test_packed_keys_of_other_lengths(dev):
