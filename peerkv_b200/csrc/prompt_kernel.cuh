@@ -55,7 +55,7 @@ constexpr uint32_t kPaColO = 256;                        // TMEM columns: S0 0, 
 // The cost axis counts thirds of a step of 128 keys x 2 row tiles (3100 cycles).  A step with one row
 // tile takes two thirds of that, an item besides its steps as long as 3 of them.
 constexpr int kPaItemCost = 1152;  // per item, = 3 x 384 keys
-constexpr int kPaMinPiece = 1536;  // no CTA gets less, = 3 x 512 keys
+constexpr int kPaMinPiece = 1024;  // no CTA gets less: a short prefix is split until a join costs more
 
 // Which CTA found which item cut (one per CTA, for the join).
 struct PromptRec {
@@ -122,7 +122,7 @@ __device__ __forceinline__ int64_t prompt_items_cost(const PromptSeq& s, int64_t
 }
 
 // Length of a CTA's piece of the cost axis: total / n_cta, a little more where the single-precision
-// quotient needs it so that n_cta pieces cover the axis.  No piece is empty: one is at least 768
+// quotient needs it so that n_cta pieces cover the axis.  No piece is empty: one is at least 512
 // long (kPaMinPiece), and what it is too long by, times n_cta, stays below that.  (A 64-bit or
 // double-precision division costs the start of every CTA some hundred cycles.)
 __device__ __forceinline__ int64_t prompt_piece(int64_t total, int n_cta) {

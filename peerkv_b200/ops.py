@@ -319,16 +319,16 @@ def quantize_kv(x: torch.Tensor, fmt: str) -> Tuple[torch.Tensor, torch.Tensor]:
 _workspace_bytes = {}
 
 
-def _prompt_workspace(device: torch.device) -> torch.Tensor:
-    """Workspace of one pkv_prompt_attention call, from torch's allocator: it belongs to the
-    current stream (or to the graph being captured), so calls on other streams and other
-    captured graphs have their own."""
+def _prompt_workspace(device: torch.device, more: int = 0) -> torch.Tensor:
+    """Workspace of one pkv_prompt_attention call and `more` bytes behind it, from torch's allocator:
+    it belongs to the current stream (or to the graph being captured), so calls on other
+    streams and other captured graphs have their own."""
     n = _workspace_bytes.get(device.index)
     if n is None:
         v = C.c_int64()
         check(_lib.lib().pkv_prompt_workspace(device.index, C.byref(v)))
         n = _workspace_bytes[device.index] = int(v.value)
-    return torch.empty(n, dtype=torch.uint8, device=device)
+    return torch.empty(n + more, dtype=torch.uint8, device=device)
 
 
 def _rows_of_heads(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -361,7 +361,7 @@ def _check_out(out: Optional[torch.Tensor], q: torch.Tensor) -> torch.Tensor:
 
 
 def _prompt_call(q, view, scale, causal, out, lse, cu_q, n_seqs, status, block_table=None, seq_lens=None, cu_k=None,
-                 more=None):
+                 more=(None, None), ws=None):
     dev = q.device
     total_q, n_heads, _ = q.shape
     st = q.stride()
@@ -370,9 +370,9 @@ def _prompt_call(q, view, scale, causal, out, lse, cu_q, n_seqs, status, block_t
                         block_table.data_ptr() if paged else None, block_table.stride(0) if paged else 0,
                         block_table.shape[1] if paged else 0, 1 if causal else 0,
                         seq_lens.data_ptr() if paged else None, None if paged else cu_k.data_ptr(),
-                        more[0].data_ptr() if more is not None else None,
-                        more[1].data_ptr() if more is not None else None, scale, 0)
-    ws = _prompt_workspace(dev)
+                        more[0], more[1], scale, 0)
+    if ws is None:
+        ws = _prompt_workspace(dev)
     check(_lib.lib().pkv_prompt_attention(dev.index, C.byref(a), out.data_ptr(), _DT[out.dtype],
                                           lse.data_ptr() if lse is not None else None, ws.data_ptr(), ws.numel(),
                                           _status_word(status, dev), _stream(dev)))
@@ -488,8 +488,11 @@ def decode_shared_prefix(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     B, Hq, D = q.shape
     scale = 1.0 / math.sqrt(D) if scale is None else scale
     pt = prefix_table if prefix_table.dim() == 2 else prefix_table[None]
-    go = torch.tensor([0, B], dtype=torch.int32, device=q.device) if group_offsets is None \
-        else _cu(group_offsets, q.device, "group_offsets")
+    if group_offsets is not None:
+        go = _cu(group_offsets, q.device, "group_offsets")
+    else:                                              # [0, B], made on the device: no copy, and capturable
+        go = torch.arange(0, B + 1, B, dtype=torch.int32, device=q.device) if B else \
+            torch.zeros(2, dtype=torch.int32, device=q.device)
     n = go.numel() - 1
     pt = _table(pt, q.device, n, "prefix_table")
     pl = _meta(prefix_lens, q.device, "prefix_lens").reshape(-1)
@@ -502,8 +505,18 @@ def decode_shared_prefix(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     out = _check_out(out, q)
     lse = torch.empty(B, Hq, dtype=torch.float32, device=q.device) if return_lse else None
     if B > 0:
-        own = partial_paged(q, k_pool, v_pool, bt, sl, scale, shard=shard)
-        _prompt_call(q, view, scale, False, out, lse, go, n, status, block_table=pt, seq_lens=pl, more=own)
+        dev = q.device
+        shard = shard or get_shard(dev, B, Hq)
+        if shard.device != dev:
+            raise PeerKVError(f"the shard context is on {shard.device}, q on {dev}")
+        qd = q if q.is_contiguous() else q.contiguous()
+        # one allocation: the join's workspace, then the own tokens' partial
+        ws = _prompt_workspace(dev, B * Hq * (D + 1) * 4)
+        o_own = ws.data_ptr() + _workspace_bytes[dev.index]
+        l_own = o_own + B * Hq * D * 4
+        a = make_args(qd, view, bt, bt.stride(0), sl, scale)
+        check(_lib.lib().pkv_decode_partial(shard._h, C.byref(a), o_own, l_own, _stream(dev)))
+        _prompt_call(q, view, scale, False, out, lse, go, n, status, block_table=pt, seq_lens=pl, more=(o_own, l_own), ws=ws)
     return (out, lse) if return_lse else out
 
 
