@@ -401,12 +401,18 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
               if (c * 32 + i >= left) sreg[c][i] = 0xff800000u;           // -inf
         }
         const uint64_t sl2 = pack_f32x2(sl, sl);
-        uint64_t ref2, sum_a, sum_b;                                       // two fp32 sums each
+        uint64_t ref2, sums;                                               // two fp32 sums
         // a row that has seen no key yet has m = -inf: 0 as the reference keeps exp2(-inf) = 0
         auto set_ref = [&]() { const float ref = m == -INFINITY ? 0.f : -m * sl; ref2 = pack_f32x2(ref, ref); };
+        auto hand_over = [&](int half) {                                   // its product can start
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_full(2 * w + half));
+        };
         float mx0 = -INFINITY, mx1 = -INFINITY;
         auto exps = [&](int half, bool with_max) {                         // 64 keys: P and its sums
-          if (half == 0) sum_a = sum_b = 0;
+          if (half == 0) sums = 0;
 #pragma unroll
           for (int c = 2 * half; c < 2 * half + 2; ++c) {
             uint32_t pk[16];
@@ -419,18 +425,15 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
                 mx0 = max3(mx0, __uint_as_float(sreg[c][i]), __uint_as_float(sreg[c][i + 1]));
                 mx1 = max3(mx1, __uint_as_float(sreg[c ^ 2][i]), __uint_as_float(sreg[c ^ 2][i + 1]));
               }
-              if (i % 4) sum_b = add_f32x2(sum_b, e2); else sum_a = add_f32x2(sum_a, e2);
+              sums = add_f32x2(sums, e2);
               const float2 e = unpack_f32x2(e2);
               pk[i / 2] = pack2<BF16>(e.x, e.y);
             }
+            // the first half goes when its stores have long arrived: waiting for them right away held the
+            // warp up (5 % of the loop)
+            if (c == 2) hand_over(0);
             tmem_st16(ts + c * 16, pk);
           }
-        };
-        auto hand_over = [&](int half) {                                   // its product can start
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(p_full(2 * w + half));
         };
         // The exponentials start with the reference of the tiles before, beside the search for this
         // tile's maximum; only if that lies more than 2^8 above are they done again (as they are
@@ -459,10 +462,9 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
             tmem_st16(to + c * 16, o);
           }
         }
-        hand_over(0);
         exps(1, false);
         hand_over(1);
-        const float2 sa = unpack_f32x2(add_f32x2(sum_a, sum_b));
+        const float2 sa = unpack_f32x2(sums);
         l += sa.x + sa.y;
       }
       if (!ok) break;
