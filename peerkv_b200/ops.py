@@ -520,10 +520,39 @@ def decode_shared_prefix(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     return (out, lse) if return_lse else out
 
 
-def _vector(t: torch.Tensor, n: int, dt, device, name: str) -> torch.Tensor:
-    if t.dtype != dt or t.device != device or t.dim() != 1 or t.numel() != n:
-        raise PeerKVError(f"{name} must be {dt} [{n}] on {device}; got {t.dtype} {tuple(t.shape)} on {t.device}")
+# The append of one decode step is a 4 us kernel behind these checks: attributes of a tensor cost 0.1 to
+# 0.2 us each, so each is read once, and devices are compared by index.
+_HALF_TYPES = (torch.float16, torch.bfloat16)
+_CODE_TYPES = (torch.int8, torch.float8_e4m3fn)
+_View1, _Base1 = KvView * 1, (C.c_int64 * 1)(0)
+
+
+def _vector(t: torch.Tensor, n: int, dt, device: int, name: str) -> torch.Tensor:
+    if t.dtype is not dt or t.get_device() != device or t.shape != (n,):
+        raise PeerKVError(f"{name} must be {dt} [{n}] on cuda:{device}; got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _append_view(i: int, kp, vp, ks, vs, dtype, n_kv_heads: int) -> KvView:
+    kdt = kp.dtype
+    if kdt is not vp.dtype or (kdt is not dtype and kdt not in _CODE_TYPES):
+        raise PeerKVError(f"pool {i}: {kdt} / {vp.dtype}; qkv's dtype, int8 or float8_e4m3fn")
+    shape, st, dev = kp.shape, kp.stride(), kp.get_device()
+    if len(shape) != 4 or shape[2] != n_kv_heads or shape[3] != HEAD_DIM or vp.shape != shape or vp.stride() != st:
+        raise PeerKVError(f"pool {i}: k and v must be [n_pages, page, {n_kv_heads}, {HEAD_DIM}] with equal strides; got "
+                          f"{tuple(shape)} and {tuple(vp.shape)}")
+    if st[3] != 1 and kp.numel() > 0:
+        raise PeerKVError("the head dimension must be contiguous")
+    if vp.get_device() != dev:
+        raise PeerKVError(f"pool {i}: v lives on {vp.device}, expected {kp.device}")
+    if kdt is dtype:
+        return KvView(kp.data_ptr(), vp.data_ptr(), None, None, _DT[kdt], n_kv_heads, HEAD_DIM, shape[1], shape[0], st[0],
+                      st[1], st[2])
+    for t in (ks, vs):
+        if t is None or t.dtype is not torch.float16 or t.shape != shape[:3] or not t.is_contiguous() or t.get_device() != dev:
+            raise PeerKVError("quantised pools need contiguous fp16 k_scale / v_scale [n_pages, page, Hkv] beside them")
+    return KvView(kp.data_ptr(), vp.data_ptr(), ks.data_ptr(), vs.data_ptr(), _DT[kdt], n_kv_heads, HEAD_DIM, shape[1],
+                  shape[0], st[0], st[1], st[2])
 
 
 def norm_rope_append(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optional[torch.Tensor], n_q_heads: int,
@@ -544,65 +573,66 @@ def norm_rope_append(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optio
     float8_e4m3fn with k_scale / v_scale [n_pages, page, Hkv] fp16; `peers` = further (k_pool,
     v_pool[, k_scale, v_scale]) on other GPUs, holding the page ids from `bases` on.
     Returns q_out.  A slot outside every pool is skipped and sets bit 2 in `status`."""
-    _require_cuda(qkv, "qkv")
-    dev = qkv.device
-    if qkv.dtype not in (torch.float16, torch.bfloat16):
-        raise PeerKVError(f"qkv must be fp16 or bf16; got {qkv.dtype}")
-    if qkv.dim() != 2 or n_q_heads < 1 or n_kv_heads < 1 or qkv.shape[1] != (n_q_heads + 2 * n_kv_heads) * HEAD_DIM:
-        raise PeerKVError(f"qkv must be [T, (n_q_heads + 2 n_kv_heads) * {HEAD_DIM}]; got {tuple(qkv.shape)}")
-    T = qkv.shape[0]
-    if T and (qkv.stride(1) != 1 or qkv.stride(0) % 8 or qkv.data_ptr() % 16):
+    dev, dt, shape, st = qkv.get_device(), qkv.dtype, qkv.shape, qkv.stride()
+    if dev < 0:
+        _require_cuda(qkv, "qkv")
+    if dt not in _HALF_TYPES:
+        raise PeerKVError(f"qkv must be fp16 or bf16; got {dt}")
+    if len(shape) != 2 or n_q_heads < 1 or n_kv_heads < 1 or shape[1] != (n_q_heads + 2 * n_kv_heads) * HEAD_DIM:
+        raise PeerKVError(f"qkv must be [T, (n_q_heads + 2 n_kv_heads) * {HEAD_DIM}]; got {tuple(shape)}")
+    T = shape[0]
+    qkv_ptr = qkv.data_ptr()
+    if T and (st[1] != 1 or st[0] % 8 or qkv_ptr % 16):
         qkv = qkv.contiguous()
+        qkv_ptr, st = qkv.data_ptr(), qkv.stride()
     if q_out is None:
-        q_out = torch.empty(T, n_q_heads, HEAD_DIM, dtype=qkv.dtype, device=dev)
-    if tuple(q_out.shape) != (T, n_q_heads, HEAD_DIM) or q_out.dtype != qkv.dtype or q_out.device != dev or \
-            (T and (q_out.stride(2) != 1 or (n_q_heads > 1 and q_out.stride(1) != HEAD_DIM))):
+        q_out = torch.empty(T, n_q_heads, HEAD_DIM, dtype=dt, device=qkv.device)
+    qs = q_out.stride()
+    if q_out.shape != (T, n_q_heads, HEAD_DIM) or q_out.dtype is not dt or q_out.get_device() != dev or \
+            (T and (qs[2] != 1 or (n_q_heads > 1 and qs[1] != HEAD_DIM))):
         raise PeerKVError(f"q_out must be [T, n_q_heads, {HEAD_DIM}] of qkv's dtype and GPU with contiguous heads")
-
-    half = 0 if inv_freq is None else inv_freq.numel()
-    positions = _vector(positions if positions.dtype == torch.int64 else positions.to(torch.int64), T, torch.int64, dev,
-                        "positions")
+    if positions.dtype is not torch.int64:
+        positions = positions.to(torch.int64)
+    positions = _vector(positions, T, torch.int64, dev, "positions")
+    half, freq_ptr, qw_ptr, kw_ptr, slot_ptr = 0, None, None, None, None
     if inv_freq is not None:
+        half = inv_freq.numel()
         inv_freq = _vector(inv_freq, half, torch.float32, dev, "inv_freq")
+        freq_ptr = inv_freq.data_ptr()
     if q_weight is not None:
-        q_weight = _vector(q_weight, HEAD_DIM, qkv.dtype, dev, "q_weight")
+        q_weight = _vector(q_weight, HEAD_DIM, dt, dev, "q_weight")
+        qw_ptr = q_weight.data_ptr()
     if k_weight is not None:
-        k_weight = _vector(k_weight, HEAD_DIM, qkv.dtype, dev, "k_weight")
+        k_weight = _vector(k_weight, HEAD_DIM, dt, dev, "k_weight")
+        kw_ptr = k_weight.data_ptr()
     views = first = None
     n_dev = 0
     if slot_mapping is not None:
         if k_pool is None or v_pool is None:
             raise PeerKVError("an append needs k_pool, v_pool and slot_mapping")
-        slot_mapping = _vector(slot_mapping if slot_mapping.dtype == torch.int64 else slot_mapping.to(torch.int64), T,
-                               torch.int64, dev, "slot_mapping")
-        pools = [(k_pool, v_pool, k_scale, v_scale)] + [tuple(p) + (None,) * (4 - len(p)) for p in peers]
-        n_dev = len(pools)
-        if len(bases) != n_dev - 1:
+        if slot_mapping.dtype is not torch.int64:
+            slot_mapping = slot_mapping.to(torch.int64)
+        slot_mapping = _vector(slot_mapping, T, torch.int64, dev, "slot_mapping")
+        slot_ptr = slot_mapping.data_ptr()
+        if k_pool.get_device() != dev:
+            raise PeerKVError(f"k_pool lives on {k_pool.device}, expected cuda:{dev}")
+        if len(bases) != len(peers):
             raise PeerKVError("every peer pool needs its first page id in bases")
-        _same_gpu(k_pool, dev, "k_pool")
-        views = (KvView * n_dev)()
-        for i, (kp, vp, ks, vs) in enumerate(pools):
-            _same_gpu(vp, kp.device, "v_pool"); _same_gpu(ks, kp.device, "k_scale"); _same_gpu(vs, kp.device, "v_scale")
-            kdt = kp.dtype
-            if kdt != vp.dtype or (kdt != qkv.dtype and kdt not in (torch.int8, torch.float8_e4m3fn)):
-                raise PeerKVError(f"pool {i}: {kdt} / {vp.dtype}; qkv's dtype, int8 or float8_e4m3fn")
-            if kdt != qkv.dtype:
-                for t in (ks, vs):
-                    if t is None or t.dtype != torch.float16 or t.shape != kp.shape[:3] or not t.is_contiguous():
-                        raise PeerKVError("quantised pools need contiguous fp16 k_scale / v_scale [n_pages, page, Hkv]")
-            if kp.dim() != 4 or kp.shape[2] != n_kv_heads or kp.shape[3] != HEAD_DIM:
-                raise PeerKVError(f"pool {i} must be [n_pages, page, {n_kv_heads}, {HEAD_DIM}]; got {tuple(kp.shape)}")
-            views[i] = paged_view(kp, vp, ks, vs)
-        if peers:
+        n_dev = 1 + len(peers)
+        home = _append_view(0, k_pool, v_pool, k_scale, v_scale, dt, n_kv_heads)
+        if n_dev == 1:
+            views, first = _View1(home), _Base1
+        else:
             from .peerkv.kv_alloc import _enable_peer_access
-            _enable_peer_access(dev, [p[0].device for p in pools[1:]])
-        first = (C.c_int64 * n_dev)(0, *[int(b) for b in bases])
+            _enable_peer_access(qkv.device, [p[0].device for p in peers])
+            more = [_append_view(i + 1, *(tuple(p) + (None,) * (4 - len(p))), dt, n_kv_heads) for i, p in enumerate(peers)]
+            views = (KvView * n_dev)(home, *more)
+            first = (C.c_int64 * n_dev)(0, *[int(b) for b in bases])
     elif k_pool is not None or v_pool is not None:
         raise PeerKVError("an append needs k_pool, v_pool and slot_mapping")
-    ptr = lambda t: t.data_ptr() if t is not None else None
-    a = _lib.AppendArgs(qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1], positions.data_ptr(), ptr(inv_freq),
-                        ptr(q_weight), ptr(k_weight), q_out.data_ptr(),
-                        q_out.stride(0) if T > 1 else n_q_heads * HEAD_DIM, ptr(slot_mapping), views, first, n_dev, T,
-                        n_q_heads, n_kv_heads, HEAD_DIM, _DT[qkv.dtype], 2 * half, 1 if interleaved else 0, eps, gain)
-    check(_lib.lib().pkv_norm_rope_append(dev.index, C.byref(a), _status_word(status, dev), _stream(dev)))
+    a = _lib.AppendArgs(qkv_ptr, st[0] if T > 1 else shape[1], positions.data_ptr(), freq_ptr, qw_ptr, kw_ptr,
+                        q_out.data_ptr(), qs[0] if T > 1 else n_q_heads * HEAD_DIM, slot_ptr, views, first, n_dev, T,
+                        n_q_heads, n_kv_heads, HEAD_DIM, _DT[dt], 2 * half, 1 if interleaved else 0, eps, gain)
+    check(_lib.lib().pkv_norm_rope_append(dev, C.byref(a), None if status is None else _status_word(status, qkv.device),
+                                          torch._C._cuda_getCurrentRawStream(dev)))
     return q_out
