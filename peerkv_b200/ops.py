@@ -113,16 +113,9 @@ def get_shard(device: torch.device, batch: int, n_q_heads: int) -> Shard:
 
 def make_args(q: torch.Tensor, kv_view: KvView, block_table: Optional[torch.Tensor],
               bt_stride: int, seq_lens: torch.Tensor, scale: float) -> DecodeArgs:
-    a = DecodeArgs()
-    a.q = q.data_ptr()
-    a.q_dtype = _DT[q.dtype]
-    a.batch, a.n_q_heads = q.shape[0], q.shape[1]
-    a.kv = kv_view
-    a.block_table = block_table.data_ptr() if block_table is not None else None
-    a.block_table_stride = bt_stride
-    a.seq_lens = seq_lens.data_ptr()
-    a.scale = float(scale)
-    return a
+    return DecodeArgs(q.data_ptr(), _DT[q.dtype], q.shape[0], q.shape[1], 0, kv_view,
+                      block_table.data_ptr() if block_table is not None else None, bt_stride, seq_lens.data_ptr(),
+                      scale, 0)
 
 
 def paged_view(k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -169,11 +162,12 @@ def _meta(t: torch.Tensor, device: torch.device, name: str) -> torch.Tensor:
     not valid on `device` must never reach a kernel."""
     if not isinstance(t, torch.Tensor):
         t = torch.as_tensor(t)
-    if t.dtype != torch.int32:
+    if t.dtype is not torch.int32:
         t = t.to(torch.int32)
     if t.device != device:
         t = t.to(device, non_blocking=True)
-    if t.dim() > 0 and t.stride(-1) != 1:
+    st = t.stride()
+    if st and st[-1] != 1:
         t = t.contiguous()
     return t
 
@@ -334,9 +328,10 @@ def _prompt_workspace(device: torch.device, more: int = 0) -> torch.Tensor:
 def _rows_of_heads(t: torch.Tensor, name: str) -> torch.Tensor:
     """[tokens, heads, 128] as the kernels read it: unit last stride, the others positive
     multiples of 8 elements, 16-byte aligned; anything else is copied."""
-    if t.dim() != 3 or t.shape[2] != HEAD_DIM:
-        raise PeerKVError(f"{name} must be [tokens, heads, {HEAD_DIM}]; got {tuple(t.shape)}")
-    n0, n1, _ = t.shape
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != HEAD_DIM:
+        raise PeerKVError(f"{name} must be [tokens, heads, {HEAD_DIM}]; got {tuple(shape)}")
+    n0, n1, _ = shape
     s0, s1, s2 = t.stride()
     ok = s2 == 1 and t.data_ptr() % 16 == 0 and (n0 <= 1 or (s0 > 0 and s0 % 8 == 0)) and \
         (n1 <= 1 or (s1 > 0 and s1 % 8 == 0))
@@ -393,19 +388,21 @@ def _cu(t, device, name) -> torch.Tensor:
 
 
 def _prompt_pool(q, k_pool, v_pool):
-    for t, n in ((k_pool, "k_pool"), (v_pool, "v_pool")):
-        _same_gpu(t, q.device, n)
+    dev, dt = q.device, q.dtype
+    _same_gpu(k_pool, dev, "k_pool")
+    _same_gpu(v_pool, dev, "v_pool")
     view = paged_view(k_pool, v_pool)
-    if k_pool.dtype != q.dtype or v_pool.dtype != q.dtype:
+    if k_pool.dtype is not dt or v_pool.dtype is not dt:
         raise PeerKVError(f"k_pool ({k_pool.dtype}), v_pool ({v_pool.dtype}) and q ({q.dtype}) must share a dtype")
     return view
 
 
 def _table(block_table, device, rows: int, name: str) -> torch.Tensor:
     bt = _meta(block_table, device, name)
-    if bt.dim() != 2 or bt.shape[0] != rows:
-        raise PeerKVError(f"{name} must be [{rows}, pages]; got {tuple(bt.shape)}")
-    return bt if bt.shape[1] > 0 else bt.new_zeros(rows, 1)
+    shape = bt.shape
+    if len(shape) != 2 or shape[0] != rows:
+        raise PeerKVError(f"{name} must be [{rows}, pages]; got {tuple(shape)}")
+    return bt if shape[1] > 0 else bt.new_zeros(rows, 1)
 
 
 def prefill_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
@@ -483,29 +480,30 @@ def decode_shared_prefix(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     describe what each sequence has of its own behind the prefix (0 tokens allowed), e.g.
     the columns of a full table behind the shared pages.  Result as decode_paged over prefix
     and own tokens: out [batch, Hq, 128], with return_lse the lse [batch, Hq].
-    The own tokens go through `shard` (see decode_paged), whose launches must not overlap."""
+    The own tokens go through `shard` (see decode_paged), whose launches must not overlap and which
+    reports their bad pages; `status` gets those of the prefixes."""
     q = _check_prompt_q(q)
     B, Hq, D = q.shape
+    dev = q.device
     scale = 1.0 / math.sqrt(D) if scale is None else scale
     pt = prefix_table if prefix_table.dim() == 2 else prefix_table[None]
     if group_offsets is not None:
-        go = _cu(group_offsets, q.device, "group_offsets")
+        go = _cu(group_offsets, dev, "group_offsets")
     else:                                              # [0, B], made on the device: no copy, and capturable
-        go = torch.arange(0, B + 1, B, dtype=torch.int32, device=q.device) if B else \
-            torch.zeros(2, dtype=torch.int32, device=q.device)
+        go = torch.arange(0, B + 1, B, dtype=torch.int32, device=dev) if B else \
+            torch.zeros(2, dtype=torch.int32, device=dev)
     n = go.numel() - 1
-    pt = _table(pt, q.device, n, "prefix_table")
-    pl = _meta(prefix_lens, q.device, "prefix_lens").reshape(-1)
+    pt = _table(pt, dev, n, "prefix_table")
+    pl = _meta(prefix_lens, dev, "prefix_lens").reshape(-1)
     if pl.numel() != n:
         raise PeerKVError(f"prefix_lens must be [{n}]; got {pl.numel()} of them")
-    bt, sl = _table(block_table, q.device, B, "block_table"), _meta(seq_lens, q.device, "seq_lens")
+    bt, sl = _table(block_table, dev, B, "block_table"), _meta(seq_lens, dev, "seq_lens")
     if sl.dim() != 1 or sl.numel() != B:
         raise PeerKVError(f"seq_lens must be [{B}]; got {tuple(sl.shape)}")
     view = _prompt_pool(q, k_pool, v_pool)
     out = _check_out(out, q)
-    lse = torch.empty(B, Hq, dtype=torch.float32, device=q.device) if return_lse else None
+    lse = torch.empty(B, Hq, dtype=torch.float32, device=dev) if return_lse else None
     if B > 0:
-        dev = q.device
         shard = shard or get_shard(dev, B, Hq)
         if shard.device != dev:
             raise PeerKVError(f"the shard context is on {shard.device}, q on {dev}")
