@@ -30,6 +30,19 @@
 // CTA, wherever the cut falls: ragged batches, causal triangles and a handful of rows over a
 // long cache are all balanced the same way.  An item that is cut leaves unnormalised (O, m, l)
 // pieces in a workspace which prompt_join_kernel adds up in a fixed order.
+//
+// What bounds it (B200, bf16, 32 q and 8 kv heads).  A step, 256 rows x 128 keys, takes the tensor
+// cores 2048 cycles and the special-function unit as many (32768 exponentials at 16 a cycle); it
+// measures 2900: a stream's scores, exponentials and product follow one another, and two streams
+// half a step apart hide most but not all of that.  8192-token prompt: 455 us (1.2 PFLOP/s, 0.75
+// of the measured burst rate of the library's large products, 0.88 of the sustained one; the
+// clock is down to 1.5 GHz under the power cap).  Short prompts and short prefixes are bound by
+// latency: 6 us from launch to the first scores (lengths, block table, first tiles, each a trip to
+// memory behind the other), 2 us an item's epilogue, 5 us the join.  A prefix of 32768 tokens for 64
+// sequences streams at 3 TB/s: its steps are compute, then the same latencies.
+// Tried and dropped: exponentials on the FMA pipe (1/16 to 1/4 of them: 4 to 25 % more cycles),
+// one S buffer for both streams with P beside it (same cycles, more code, ragged batches 10 % slower),
+// one warp issuing both streams' products (waits and issue between them took as long as they did).
 #pragma once
 #include "decode_kernel.cuh"
 #include "tcgen05.cuh"
@@ -52,10 +65,11 @@ constexpr int kPaMaxCtas = 256;
 constexpr int kPaSoftmaxRegs = 208;
 constexpr int kPaOtherRegs = 80;
 constexpr uint32_t kPaColO = 256;                        // TMEM columns: S0 0, S1 128, O0 256, O1 384
-// The cost axis counts thirds of a step of 128 keys x 2 row tiles (3100 cycles).  A step with one row
-// tile takes two thirds of that, an item besides its steps as long as 3 of them.
+// The cost axis counts thirds of a key of a step with two row tiles.  A step with one row
+// tile takes two thirds of that; what an item takes besides its steps (first scores, epilogue) is
+// weighted like three steps (192 keys instead of 384 left ragged batches 10 % out of balance).
 constexpr int kPaItemCost = 1152;  // per item, = 3 x 384 keys
-constexpr int kPaMinPiece = 1024;  // no CTA gets less: a short prefix is split until a join costs more
+constexpr int kPaMinPiece = 1024;  // no CTA gets less (2048-token prefix: 34 us; 35 with 768, 36 with 1536)
 
 // Which CTA found which item cut (one per CTA, for the join).
 struct PromptRec {
