@@ -308,9 +308,12 @@ class PromptStep:
              cu_seqlens: torch.Tensor, seq_lens: torch.Tensor) -> torch.Tensor:
         """tokens, positions, slot_mapping [T] int64 (page * page size + offset of this GPU's pools);
         cu_seqlens [n + 1] int32 offsets of the sequences in them; seq_lens [n] int32 tokens of
-        each in the cache, the new ones included -> logits [n, vocab]."""
+        each in the cache, the new ones included -> logits [n, vocab], 0 for a sequence without
+        new tokens."""
         g, T = self.g, tokens.shape[0]
         dt = self.w.embed.dtype
+        if T == 0:
+            return torch.zeros(cu_seqlens.shape[0] - 1, g.vocab, dtype=dt, device=self.dev)
         x = self.w.embed.index_select(0, tokens)
         h = torch.empty_like(x)
         act = torch.empty(T, g.ffn, dtype=dt, device=self.dev)
@@ -327,4 +330,7 @@ class PromptStep:
             swiglu(torch.matmul(h, lw.w_gate_up), act)
             delta = torch.matmul(act, lw.w_down)
         add_rmsnorm(x, delta, self.w.final_norm, h, g.rms_eps)
-        return torch.matmul(h.index_select(0, cu_seqlens[1:].long() - 1), self.w.lm_head)
+        # (clamped: an index outside h would end the process, not only the call)
+        last = h.index_select(0, (cu_seqlens[1:].long() - 1).clamp_(0, T - 1))
+        last.masked_fill_((cu_seqlens[1:] <= cu_seqlens[:-1])[:, None], 0.0)
+        return torch.matmul(last, self.w.lm_head)

@@ -137,6 +137,27 @@ def test_decode_behind_a_shared_prefix(dev):
     assert ds.shard.status() == 0
 
 
+def test_sequences_without_new_tokens(dev):
+    """A padded batch: first, middle and last sequences that add nothing give logits 0 and leave the
+    others' as they are; a batch that adds nothing at all gives 0 everywhere."""
+    from peerkv_b200.decoder import PromptStep
+    g, w = model(dev)
+    gen = torch.Generator().manual_seed(17)
+    lens = [0, 21, 0, 0, 5, 0]
+    seqs = [torch.randint(0, g.vocab, (n,), generator=gen) for n in lens]
+    kept = [1, 4]
+    some, tab = caches(g, [lens[i] for i in kept], 0, dev)
+    ref = PromptStep(g, w, some, dev).step(*packed([seqs[i] for i in kept], [0, 0], [lens[i] for i in kept], tab, dev))
+    every, tab = caches(g, lens, 0, dev)
+    got = PromptStep(g, w, every, dev).step(*packed(seqs, [0] * 6, lens, tab, dev))
+    close(got[kept], ref)
+    assert (got[[0, 2, 3, 5]] == 0).all()
+    none = torch.zeros(0, dtype=torch.int64, device=dev)
+    zero = torch.zeros(7, dtype=torch.int32, device=dev)
+    out = PromptStep(g, w, every, dev).step(none, none, none, zero, zero[1:])
+    assert out.shape == (6, g.vocab) and (out == 0).all()
+
+
 def test_a_group_and_a_prefix_are_refused(dev):
     from peerkv_b200 import PeerKVError
     from peerkv_b200.decoder import DecodeStep
