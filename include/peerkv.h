@@ -427,7 +427,8 @@ int pkv_swiglu(int device, const void* gate_up, void* out, int32_t rows, int32_t
  * What the pool holds behind a sequence's last token is never used, not even when it is
  * NaN; the tokens of a sequence must be finite in V, since a matrix instruction multiplies a
  * hidden key of the same 128-key tile by a weight of 0.  n_q_heads / n_kv_heads <= 128.  A
- * page id outside the pool is read as page 0 and sets PKV_ST_BAD_PAGE. */
+ * page id outside the pool is read as page 0 and sets PKV_ST_BAD_PAGE.  Offsets and lengths
+ * are clamped: to total_q rows, and to the tokens that a block-table row has room for. */
 typedef struct pkv_prompt_args {
   const void* q;
   int64_t q_token_stride;

@@ -305,7 +305,6 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   float2* xml = reinterpret_cast<float2*>(misc + 640);                         // behind the first sequence at 592
   static_assert(sizeof(PromptSeq) <= 48, "first sequence");
 
-
   if (threadIdx.x == 0) {
     for (int i = 0; i < kPaSlots; ++i) { mbar_init(full(i), 1); mbar_init(empty(i), 2); }
     mbar_init(q_full, 1); mbar_init(q_empty, 2); mbar_init(done, 2);
@@ -877,8 +876,8 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         };
         // Two row tiles: both streams take every tile, and they issue in turn: O_0 (+)= P_0 V and the
         // next S_0, then the same of stream 1.  Left alone they fall into step, and the
-        // exponentials of both wait for the tensor cores and then compete (measured: 4300 cycles a
-        // step instead of 3100).  One row tile: stream w takes tiles w, w + 2, ..., and lets the
+        // exponentials of both wait for the tensor cores and then compete (4300 cycles a step
+        // instead of 3100 when this was put in).  One row tile: stream w takes tiles w, w + 2, ..., and lets the
         // others pass, so that no slot is filled again before both have seen it.
         const bool two = uniform(wk.two);
         const int ahead = two ? 1 : 2;                  // scores a stream is ahead of its values

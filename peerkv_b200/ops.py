@@ -541,8 +541,8 @@ def _append_view(i: int, kp, vp, ks, vs, dtype, n_kv_heads: int) -> KvView:
                           f"{tuple(shape)} and {tuple(vp.shape)}")
     if st[3] != 1 and kp.numel() > 0:
         raise PeerKVError("the head dimension must be contiguous")
-    if vp.get_device() != dev:
-        raise PeerKVError(f"pool {i}: v lives on {vp.device}, expected {kp.device}")
+    if dev < 0 or vp.get_device() != dev:
+        raise PeerKVError(f"pool {i}: k and v must be CUDA tensors on one GPU; got {kp.device} and {vp.device}")
     if kdt is dtype:
         return KvView(kp.data_ptr(), vp.data_ptr(), None, None, _DT[kdt], n_kv_heads, HEAD_DIM, shape[1], shape[0], st[0],
                       st[1], st[2])
@@ -622,8 +622,8 @@ def norm_rope_append(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optio
             views, first = _View1(home), _Base1
         else:
             from .peerkv.kv_alloc import _enable_peer_access
-            _enable_peer_access(qkv.device, [p[0].device for p in peers])
             more = [_append_view(i + 1, *(tuple(p) + (None,) * (4 - len(p))), dt, n_kv_heads) for i, p in enumerate(peers)]
+            _enable_peer_access(qkv.device, [p[0].device for p in peers])
             views = (KvView * n_dev)(home, *more)
             first = (C.c_int64 * n_dev)(0, *[int(b) for b in bases])
     elif k_pool is not None or v_pool is not None:

@@ -120,6 +120,14 @@ def test_structs_are_the_header_s(tmp_path):
             assert int(got[f"{name}.{f}"]) == getattr(cls, f).offset
 
 
+def test_python_refuses_host_pools():
+    """Every pool of an append goes through one check; a host pointer must not reach the kernel."""
+    from peerkv_b200 import PeerKVError, ops
+    pool = torch.zeros(3, 16, 2, 128).bfloat16()
+    with pytest.raises(PeerKVError, match="CUDA"):
+        ops._append_view(1, pool, pool, None, None, torch.bfloat16, 2)
+
+
 def test_python_refuses_cpu_tensors():
     from peerkv_b200 import PeerKVError, ops
     q, pool = torch.zeros(2, 8, 128).bfloat16(), torch.zeros(3, 16, 2, 128).bfloat16()
@@ -173,6 +181,10 @@ def test_python_refuses_on_the_gpu():
                                       i(0, 1, 2).long()), "n_pages"),
         (lambda: ops.norm_rope_append(z(3, 1536), i(0, 0, 0).long(), None, 8, 2, None, pool, pool, i(0, 1, 2).long(),
                                       peers=[(pool, pool)]), "bases"),
+        (lambda: ops.norm_rope_append(z(3, 1536), i(0, 0, 0).long(), None, 8, 2, None, pool, pool, i(0, 1, 2).long(),
+                                      peers=[(pool.cpu(), pool.cpu())], bases=[3]), "CUDA"),
+        (lambda: ops.norm_rope_append(z(3, 1536), i(0, 0, 0).long(), None, 8, 2, None, pool.cpu(), pool.cpu(),
+                                      i(0, 1, 2).long()), "expected cuda"),
     ]
     for n, (call, word) in enumerate(bad):
         with pytest.raises(PeerKVError, match=word):
