@@ -84,7 +84,9 @@ typedef struct pkv_kv_view {
  *                sequence order; NULL means page j of sequence b is b*block_table_stride + j
  *   seq_lens     [batch] int32 tokens of each sequence that live in THIS shard
  *                (0 allowed; only a sequence's last listed page may be partial)
- *   scale        softmax scale (the reference default is 1/sqrt(head_dim)) */
+ *   scale        softmax scale (the reference default is 1/sqrt(head_dim))
+ *   early_dependent  1: the kernel behind this one may take SMs as they become free (see more_late
+ *                in pkv_prompt_args; of no use for anything else) */
 typedef struct pkv_decode_args {
   const void* q;
   int32_t q_dtype;
@@ -96,7 +98,7 @@ typedef struct pkv_decode_args {
   int64_t block_table_stride;
   const int32_t* seq_lens;
   float scale;
-  int32_t reserved1;
+  int32_t early_dependent;
 } pkv_decode_args;
 
 const char* pkv_last_error(void);
@@ -423,6 +425,9 @@ int pkv_swiglu(int device, const void* gate_up, void* out, int32_t rows, int32_t
  *               gives O = 0 and lse = -inf
  *   o_more, lse_more: NULL, or one more partial of the same rows ([total_q, n_q_heads, 128]
  *               fp32 normalised, [total_q, n_q_heads] natural log) to fold into the result
+ *   more_late      1: o_more and lse_more are written by the pkv_decode_partial right before this
+ *               call in the stream, which was given early_dependent; all else this call reads or
+ *               writes was finished before that one.  The two then overlap at their seam
  *   scale          finite and > 0
  * What the pool holds behind a sequence's last token is never used, not even when it is
  * NaN; the tokens of a sequence must be finite in V, since a matrix instruction multiplies a
@@ -448,7 +453,7 @@ typedef struct pkv_prompt_args {
   const float* o_more;
   const float* lse_more;
   float scale;
-  int32_t reserved0;
+  int32_t more_late;
 } pkv_prompt_args;
 
 /* Bytes of workspace one call needs on `device` (about 40 MB on a B200; 256-byte aligned device

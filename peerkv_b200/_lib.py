@@ -41,7 +41,7 @@ class DecodeArgs(C.Structure):
     _fields_ = [("q", C.c_void_p), ("q_dtype", C.c_int32), ("batch", C.c_int32),
                 ("n_q_heads", C.c_int32), ("reserved0", C.c_int32), ("kv", KvView),
                 ("block_table", C.c_void_p), ("block_table_stride", C.c_int64),
-                ("seq_lens", C.c_void_p), ("scale", C.c_float), ("reserved1", C.c_int32)]
+                ("seq_lens", C.c_void_p), ("scale", C.c_float), ("early_dependent", C.c_int32)]
 
 
 class PromptArgs(C.Structure):
@@ -50,7 +50,7 @@ class PromptArgs(C.Structure):
                 ("cu_seqlens_q", C.c_void_p), ("kv", KvView), ("block_table", C.c_void_p),
                 ("block_table_stride", C.c_int64), ("block_table_cols", C.c_int32), ("causal", C.c_int32),
                 ("seq_lens", C.c_void_p), ("cu_seqlens_k", C.c_void_p), ("o_more", C.c_void_p),
-                ("lse_more", C.c_void_p), ("scale", C.c_float), ("reserved0", C.c_int32)]
+                ("lse_more", C.c_void_p), ("scale", C.c_float), ("more_late", C.c_int32)]
 
 
 class AppendArgs(C.Structure):

@@ -345,6 +345,7 @@ int launch_decode(pkv_shard* s, const pkv_decode_args* a, const LaunchOut& lo, c
   p.o_ll = lo.o_ll;
   p.lse_ll = lo.lse_ll;
   p.force_empty = kv.n_pages > 0 ? 0 : 1;
+  p.early_dependent = a->early_dependent ? 1 : 0;
   p.trace = s->trace;
   p.stats = reinterpret_cast<unsigned long long*>(reinterpret_cast<uint8_t*>(s->status) + 64);
   p.k_scale = kv.k_scale;
@@ -1407,6 +1408,7 @@ extern "C" int pkv_prompt_attention(int device, const pkv_prompt_args* a, void* 
   p.causal = a->causal ? 1 : 0;
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.out = out; p.out_dtype = out_dtype; p.lse = lse; p.o_more = a->o_more; p.lse_more = a->lse_more;
+  p.more_late = a->o_more && a->more_late ? 1 : 0;
   uint8_t* wsb = static_cast<uint8_t*>(workspace);
   p.part_o = reinterpret_cast<float4*>(wsb + ws.o);
   p.part_ml = reinterpret_cast<float2*>(wsb + ws.ml);

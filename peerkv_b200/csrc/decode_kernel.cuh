@@ -73,6 +73,7 @@ struct DecodeParams {
   int head_major;      // 1: pool dims are (d, tok, head, page); 0: (d, head, tok, page)
   int n_cta_x;
   int force_empty;     // 1: the pool holds no page; every sequence counts as empty here
+  int early_dependent; // 1: the kernel behind this one may take its SMs as they become free
   float scale_log2;    // softmax scale * log2(e)
   float* part_o;       // [slots][Hq][128]
   float* part_ml;      // [slots][Hq][2]  (m in log2 units, l)
@@ -659,8 +660,10 @@ decode_partial_kernel(const __grid_constant__ CUtensorMap tm_k,
   // line; below it everything the previous kernel wrote is visible.  The kernel does NOT
   // trigger its own dependents early: CTAs placed on whichever SM frees first land on other
   // SMs than last time, and the split of the tile list, which learns per CTA index how fast
-  // its SM streams, then balances worse (measured: 5 % slower steps).
+  // its SM streams, then balances worse (measured: 5 % slower steps).  That holds for a decode
+  // kernel behind a decode kernel; prompt attention behind one learns nothing and gains its start.
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (p.early_dependent) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint64_t epoch = (p.epoch_base ? *reinterpret_cast<const volatile uint64_t*>(p.epoch_base) : 0ull) +
                          p.epoch_rel;
   int* bound = reinterpret_cast<int*>(sgen + L::kBoundOff);

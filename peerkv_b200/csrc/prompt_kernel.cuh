@@ -99,6 +99,7 @@ struct PromptParams {
   float* lse;                  // [total_q][n_q_heads] or null
   const float* o_more;         // one more partial of the same rows to fold in, or null
   const float* lse_more;
+  int more_late;               // o_more, lse_more come from the kernel before this one, which may still run
   float4* part_o;              // workspace: [2 * CTAs][32][256]
   float2* part_ml;             // [2 * CTAs][256]
   PromptRec* rec;              // [CTAs + 1]; rec[CTAs].kt0 = CTAs in use
@@ -317,8 +318,10 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
   }
   if (warp == 8) tmem_alloc(smem_u32(tmem_word), 512);
   if (warp == 9 && lane == 0) { prefetch_tensormap(&qmap); prefetch_tensormap(&kmap); prefetch_tensormap(&vmap); }
-  // Launched with programmatic stream serialisation: nothing of global memory is read above.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // Launched with programmatic stream serialisation: nothing of global memory is read above.  With
+  // more_late only the other partial of the rows is still in the making: the kernel starts on SMs
+  // that its maker has left, and waits where it needs that partial or writes a result.
+  if (!p.more_late) asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- this CTA's piece of the cost axis ----
@@ -518,6 +521,7 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         const float m2 = m == -INFINITY ? -INFINITY : m * sl;           // base-2 units
         float wa = l > 0.f ? 1.f / l : 0.f, wb = 0.f;
         if (l != l) wa = l;                                            // NaN scores stay NaN
+        if (p.more_late) asm volatile("griddepcontrol.wait;" ::: "memory");
         if (whole && valid) {
           float lse2 = l > 0.f ? m2 + log2f(l) : (l != l ? l : -INFINITY);
           if (p.o_more) {
@@ -908,6 +912,8 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       mbar_wait_bounded(done, 0, kPollLimit);
     }
   }
+  // (the join takes the end of this kernel for the end of the one before)
+  if (p.more_late) asm volatile("griddepcontrol.wait;" ::: "memory");
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && *abort_flag && p.status) atomicOr(p.status, kStPipeTimeout);

@@ -112,10 +112,10 @@ def get_shard(device: torch.device, batch: int, n_q_heads: int) -> Shard:
 
 
 def make_args(q: torch.Tensor, kv_view: KvView, block_table: Optional[torch.Tensor],
-              bt_stride: int, seq_lens: torch.Tensor, scale: float) -> DecodeArgs:
+              bt_stride: int, seq_lens: torch.Tensor, scale: float, early_dependent: int = 0) -> DecodeArgs:
     return DecodeArgs(q.data_ptr(), _DT[q.dtype], q.shape[0], q.shape[1], 0, kv_view,
                       block_table.data_ptr() if block_table is not None else None, bt_stride, seq_lens.data_ptr(),
-                      scale, 0)
+                      scale, early_dependent)
 
 
 def paged_view(k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -365,7 +365,7 @@ def _prompt_call(q, view, scale, causal, out, lse, cu_q, n_seqs, status, block_t
                         block_table.data_ptr() if paged else None, block_table.stride(0) if paged else 0,
                         block_table.shape[1] if paged else 0, 1 if causal else 0,
                         seq_lens.data_ptr() if paged else None, None if paged else cu_k.data_ptr(),
-                        more[0], more[1], scale, 0)
+                        more[0], more[1], scale, 0 if more[0] is None else 1)
     if ws is None:
         ws = _prompt_workspace(dev)
     check(_lib.lib().pkv_prompt_attention(dev.index, C.byref(a), out.data_ptr(), _DT[out.dtype],
@@ -512,7 +512,9 @@ def decode_shared_prefix(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
         ws = _prompt_workspace(dev, B * Hq * (D + 1) * 4)
         o_own = ws.data_ptr() + _workspace_bytes[dev.index]
         l_own = o_own + B * Hq * D * 4
-        a = make_args(qd, view, bt, bt.stride(0), sl, scale)
+        # nothing comes between the two launches: the second starts while the first ends (graph of b4 / b64 with
+        # a prefix of 2048 / 32768 tokens: 33.4 -> 25.4 us, 106.2 -> 99.7 us)
+        a = make_args(qd, view, bt, bt.stride(0), sl, scale, 1)
         check(_lib.lib().pkv_decode_partial(shard._h, C.byref(a), o_own, l_own, _stream(dev)))
         _prompt_call(q, view, scale, False, out, lse, go, n, status, block_table=pt, seq_lens=pl, more=(o_own, l_own), ws=ws)
     return (out, lse) if return_lse else out
