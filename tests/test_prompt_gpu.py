@@ -242,6 +242,49 @@ def test_captured_and_replayed(dev):
     del g1, g2
 
 
+def test_shared_prefix_sees_what_was_written_right_before(dev):
+    """Every input is overwritten in place right before each call, eagerly and in a replayed graph:
+    the prefix kernel, which starts before the decode kernel has ended, reads none of the old values."""
+    from peerkv_b200 import ops
+    cases = [prefix_case([(size, plen)], 40, 8, 2, 16, torch.bfloat16, 60 + i)
+             for i, (size, plen) in enumerate([(9, 1500), (9, 700), (9, 1501), (9, 33)])]
+    pages = max(c[1].shape[0] for c in cases)
+    cols = [max(c[j].shape[1] for c in cases) for j in (3, 5)]
+
+    def pad(x, shape):
+        y = torch.zeros(shape, dtype=x.dtype)
+        y[tuple(slice(n) for n in x.shape)] = torch.nan_to_num(x) if x.is_floating_point() else x
+        return y.to(dev)
+    sets = [[c[0].to(dev), pad(c[1], (pages, *c[1].shape[1:])), pad(c[2], (pages, *c[2].shape[1:])),
+             pad(c[3], (1, cols[0])), c[4].to(dev), pad(c[5], (9, cols[1])), c[6].to(dev)] for c in cases]
+    live = [x.clone() for x in sets[0]]
+    go = cases[0][7].to(dev)
+    shard = ops.Shard(dev, 9, 8)
+
+    def refill(i):
+        for x, y in zip(live, sets[i % 4]):
+            x.copy_(y)
+
+    def call():
+        return ops.decode_shared_prefix(*live, group_offsets=go, return_lse=True, shard=shard)
+    got = []
+    for i in range(24):
+        refill(i)
+        got.append(call())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = call()
+    for i in range(24):
+        refill(i)
+        graph.replay()
+        got.append([x.clone() for x in res])
+    torch.cuda.synchronize()
+    for i, (out, lse) in enumerate(got):
+        assert_close(out, lse, *cases[i % 4][8], torch.bfloat16, cases[i % 4][9])
+    del graph
+
+
 def test_bad_pages_set_the_status_bit(dev):
     from peerkv_b200 import ops
     q, k, v, table, sl, cu, ref, most = paged_case([(40, 300), (16, 64)], 8, 2, 16, torch.bfloat16, 61)
