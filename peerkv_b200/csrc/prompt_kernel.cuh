@@ -928,7 +928,9 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
 // tasks of (item, 8 of the 128 values); one thread per row, so a piece's values come in
 // 4 KB runs.  The pieces are a few MB that were written a moment ago: L2.
 constexpr int kPjTasks = 16;
-constexpr int kPjBatch = 8;        // pieces in flight per thread: a join is a few trips to the L2, not one per piece
+// Pieces in flight per thread: a join is a few trips to the L2, not one per piece.  (4: packed short prompts
+// 28.2 us instead of 29.2, but 64 sequences behind 32768 tokens, 18 pieces an item, 103.6 instead of 101.7.)
+constexpr int kPjBatch = 8;
 __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptParams p, int n_grid) {
   __shared__ int64_t s_a[kPaMaxCtas];
   __shared__ int s_kt0[kPaMaxCtas], s_kt1[kPaMaxCtas], s_n[kPaMaxCtas];
