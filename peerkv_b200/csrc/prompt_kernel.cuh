@@ -389,12 +389,17 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
     const uint32_t lane_base = tmem + ((uint32_t)(warp & 3) << 21);      // lane 32 * (warp % 4)
     const uint32_t ts = lane_base + w * 128, to = lane_base + kPaColO + w * 128;
     const int tok_in = row / p.group;
-    const float sl = p.scale_log2;
     uint32_t n_s = 0, n_o = 0, n_x = 0;                                   // barrier phases used
     while (active && take()) {
       const bool two = wk.two;
       const int tok = (two ? w * p.tok_tile : 0) + tok_in;               // token of this row in the item
       const int steps = two ? wk.n_tiles : (wk.n_tiles + 1 - w) >> 1;    // one row tile: alternate KV tiles
+      // The row is a query of this item.  The others hold the queries behind it or, where the group does not
+      // divide 128, what the last call left in shared memory: scaled by 0 they run along and never move their
+      // warp's reference (which would round the rows beside them otherwise from call to call).  Costs 1 % on
+      // long prompts; a test in the condition cost 3 to 6 %.
+      const bool valid = tok < wk.n_tok && row < p.tok_tile * p.group;
+      const float sl = valid ? p.scale_log2 : 0.f;
       // keys [0, lim) are visible to this row
       const int lim = p.causal ? min(wk.len, wk.lim0 + tok) : wk.len;
       int left = lim - (wk.kt0 + (two ? 0 : w)) * kPaKeys;               // of them, in and behind this tile
@@ -515,7 +520,6 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         }
       }
       if (two || w == 0) {
-        const bool valid = tok < wk.n_tok && row < p.tok_tile * p.group;
         const bool whole = wk.slot < 0;
         const int64_t orow = (int64_t)(wk.q0 + tok) * p.n_q_heads + wk.h * p.group + (row - tok_in * p.group);
         const float m2 = m == -INFINITY ? -INFINITY : m * sl;           // base-2 units
