@@ -360,7 +360,9 @@ int launch_decode(pkv_shard* s, const pkv_decode_args* a, const LaunchOut& lo, c
   p.grp_slot0 = s->grp_slot0;
   p.sib_slot0 = s->grp_slot0 / pkv::kMaxWph;
   p.unit_slot0 = s->n_slots - s->max_batch;
-  if (s->obs[0] && n_cta_x <= pkv::kMaxCtas) {
+  // (Not with early_dependent: a call that ends in prompt attention keeps nothing between calls, and its
+  // sums are cut where the lengths alone say.)
+  if (s->obs[0] && n_cta_x <= pkv::kMaxCtas && !a->early_dependent) {
     p.obs_read = s->obs[s->obs_parity];
     p.obs_write = s->obs[s->obs_parity ^ 1];
     s->obs_parity ^= 1;
