@@ -532,10 +532,10 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
             const float b2 = p.lse_more[orow] * 1.4426950408889634f;
             const float top = fmaxf(lse2, b2);
             const float ea = lse2 == -INFINITY ? 0.f : exp2f(lse2 - top), eb = b2 == -INFINITY ? 0.f : exp2f(b2 - top);
-            const float s = ea + eb, inv = s > 0.f ? 1.f / s : 0.f;
+            const float s = ea + eb, inv = s > 0.f ? 1.f / s : (s != s ? s : 0.f);     // a NaN on either side stays one
             wa *= ea * inv;
             wb = eb * inv;
-            lse2 = s > 0.f ? top + log2f(s) : -INFINITY;
+            lse2 = s > 0.f ? top + log2f(s) : (s != s ? s : -INFINITY);
           }
           if (p.lse) p.lse[orow] = lse2 * 0.6931471805599453f;
         }
