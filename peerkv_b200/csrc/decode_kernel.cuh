@@ -26,6 +26,7 @@
 // with movmatrix.  Decode is HBM-bound: the tensor cores are used because the
 // CUDA-core form needs ~8 issue cycles per KV row, more than HBM leaves.
 #pragma once
+#include <cfloat>
 #include "ptx.cuh"
 
 namespace pkv {
@@ -217,10 +218,11 @@ __device__ __forceinline__ void store_out4(void* out, int dtype, int64_t idx, fl
 }
 
 // Online-softmax fold of one slot (running max m in log2 units, sum l, unnormalised row o)
-// into the accumulator; a slot with m = -inf carries no tokens and is skipped.
+// into the accumulator; a slot with m = -inf carries no weight and is skipped, unless its sum says
+// that its scores were NaN.
 __device__ __forceinline__ void fold_slot(float& M, float& L, float4& acc, float m, float l,
                                           const float4& o) {
-  if (m == -INFINITY) return;
+  if (m == -INFINITY && l == l) return;
   const float mn = fmaxf(M, m);
   const float ca = fast_exp2(M - mn), cs = fast_exp2(m - mn);
   L = L * ca + l * cs;
@@ -370,11 +372,11 @@ __device__ __forceinline__ bool combine_heads(const DecodeParams& p, uint32_t ta
 #pragma unroll
   for (int i = 0; i < NH; ++i) {
     if (i < nh) {
-      const float inv = L[i] > 0.f ? 1.f / L[i] : 0.f;
+      const float inv = L[i] > 0.f ? 1.f / L[i] : (L[i] != L[i] ? L[i] : 0.f);       // NaN stays NaN
       float4 v = acc[i];
       v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv;
       const int64_t idx = ((int64_t)b * p.n_q_heads + qh0 + i) * kHeadDim + lane * 4;
-      const float lse = L[i] > 0.f ? (M[i] + log2f(L[i])) * 0.6931471805599453f : -INFINITY;
+      const float lse = L[i] > 0.f ? (M[i] + log2f(L[i])) * 0.6931471805599453f : (L[i] != L[i] ? L[i] : -INFINITY);
       const int64_t row = (int64_t)b * p.n_q_heads + qh0 + i;
       if (p.out) store_out4(p.out, p.out_dtype, idx, v);
       if (p.o_part) *reinterpret_cast<float4*>(p.o_part + idx) = v;
@@ -1045,7 +1047,8 @@ decode_partial_kernel(const __grid_constant__ CUtensorMap tm_k,
     float o[8][4];
 #pragma unroll
     for (int j = 0; j < 8; ++j) { o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f; }
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    // From the lowest finite value on: where every score so far is -inf, exp2(-inf - m) is 0 and not NaN.
+    float m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;
     const int n_seq_tiles = prefix[s + 1] - prefix[s];
 
     const int tile_base = prefix[s];
@@ -1235,6 +1238,8 @@ decode_partial_kernel(const __grid_constant__ CUtensorMap tm_k,
         l0 += __shfl_xor_sync(0xffffffffu, l0, off);
         l1 += __shfl_xor_sync(0xffffffffu, l1, off);
       }
+      if (m0 == -FLT_MAX) m0 = -INFINITY;
+      if (m1 == -FLT_MAX) m1 = -INFINITY;
       const int h0 = 2 * t, h1 = 2 * t + 1;
       // Two warps per head (1-byte pools): the second warp parks its partial in a slot of
       // its own and hands over; the first folds it into its registers, so the CTA leaves

@@ -174,14 +174,19 @@ __global__ void __launch_bounds__(256) merge_partials_kernel(const MergeParams p
       acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
     }
     store_out4(p.out, p.out_dtype, (int64_t)row * kHeadDim + lane * 4, acc);
-    if (p.lse_out && lane == 0) p.lse_out[row] = wsum > 0.f ? M + __logf(wsum) : -INFINITY;
+    if (p.lse_out && lane == 0) p.lse_out[row] = wsum > 0.f ? M + __logf(wsum) : (wsum != wsum ? wsum : -INFINITY);
     return;
   }
   float L = -INFINITY;
-  for (int i = 0; i < p.n_parts; ++i) L = fmaxf(L, __ldcg(p.lse_parts + i * p.lse_stride + row));
+  bool nan = false;                       // the maximum passes a NaN over; the weights below do not
+  for (int i = 0; i < p.n_parts; ++i) {
+    const float li = __ldcg(p.lse_parts + i * p.lse_stride + row);
+    L = fmaxf(L, li);
+    nan = nan || li != li;
+  }
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float wsum = 0.f;
-  if (L > -INFINITY) {
+  if (L > -INFINITY || nan) {
     for (int i = 0; i < p.n_parts; ++i) {
       const float li = __ldcg(p.lse_parts + i * p.lse_stride + row);
       if (li == -INFINITY) continue;
@@ -196,7 +201,7 @@ __global__ void __launch_bounds__(256) merge_partials_kernel(const MergeParams p
   }
   const int64_t idx = (int64_t)row * kHeadDim + lane * 4;
   store_out4(p.out, p.out_dtype, idx, acc);
-  if (p.lse_out && lane == 0) p.lse_out[row] = L > -INFINITY ? L + __logf(wsum) : -INFINITY;
+  if (p.lse_out && lane == 0) p.lse_out[row] = L > -INFINITY || nan ? L + __logf(wsum) : -INFINITY;
 }
 
 // Per-row absmax quantiser (one warp per row of 128 values, 4 per lane).

@@ -205,7 +205,8 @@ __global__ void __launch_bounds__(kPfThreads) prefill_partial_kernel(const Prefi
 
   l0 += __shfl_xor_sync(0xffffffffu, l0, 1); l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
   l1 += __shfl_xor_sync(0xffffffffu, l1, 1); l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-  const float inv0 = l0 > 0.f ? 1.f / l0 : 0.f, inv1 = l1 > 0.f ? 1.f / l1 : 0.f;
+  const float inv0 = l0 > 0.f ? 1.f / l0 : 0.f, inv1 = l1 > 0.f ? 1.f / l1 : 0.f;      // (a NaN row's o is NaN)
+  auto lse = [](float m, float l) { return l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : (l != l ? l : -INFINITY); };
   const int ra = row0 + wr + g, rb = ra + 8;
   const int64_t base = ((int64_t)b * p.n_q_heads + h) * p.sq;
 #pragma unroll
@@ -215,8 +216,8 @@ __global__ void __launch_bounds__(kPfThreads) prefill_partial_kernel(const Prefi
     if (rb < p.sq) *reinterpret_cast<float2*>(p.o_part + (base + rb) * kHeadDim + d) = make_float2(o[j][2] * inv1, o[j][3] * inv1);
   }
   if (t == 0) {
-    if (ra < p.sq) p.lse_part[base + ra] = l0 > 0.f ? (m0 + log2f(l0)) * 0.6931471805599453f : -INFINITY;
-    if (rb < p.sq) p.lse_part[base + rb] = l1 > 0.f ? (m1 + log2f(l1)) * 0.6931471805599453f : -INFINITY;
+    if (ra < p.sq) p.lse_part[base + ra] = lse(m0, l0);
+    if (rb < p.sq) p.lse_part[base + rb] = lse(m1, l1);
   }
 }
 
