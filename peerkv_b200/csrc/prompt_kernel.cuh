@@ -21,10 +21,15 @@
 //
 // Sums.  Scores, maxima, sums and O are fp32.  P is rounded to the 16-bit type of V, as the
 // matrix instruction wants both operands alike; the row sum adds the unrounded values.  The
-// rounding costs an output as much as its own last rounding does (2^-9 relative per weight,
-// independent signs), half of the error budget of a 16-bit output.  The reference of the
-// exponentials moves only when a row's maximum has grown by more than 2^8: until then P
-// stays <= 256 and O need not be touched; l and lse use the same reference, so nothing is lost.
+// rounding costs an output as much as its own last rounding does (2^-9 relative per weight in bf16, 2^-12
+// in fp16 on average, independent signs), half of the error budget of a 16-bit output.  (The kernel for dense
+// tensors, prefill_kernel.cuh, sends a bf16 P as two terms: its result is an fp32 partial.  Here that
+// would be half as many products again on the pipe that bounds a step, for an output that is
+// rounded to 16 bits itself.)  The reference of the exponentials moves only when a row's maximum has grown
+// by more than 2^8: until then O need not be touched; l and lse use the same reference, so nothing
+// is lost.  fp16 ends at 2^-24, and behind one dominant key the many small weights can be the output: there
+// the reference is lifted by 2^7, so that the row's largest weight stands between 2^7 and 2^15 and a small one
+// keeps its 11 bits down to 2^-21 of it and is off by at most 2^-32 of it below.  bf16 has fp32's range.
 //
 // Work split.  The KV tiles of all items form one list that is cut into equal pieces, one per
 // CTA, wherever the cut falls: ragged batches, causal triangles and a handful of rows over a
@@ -64,6 +69,8 @@ constexpr int kPaMaxCtas = 256;
 // 384 threads x 168 registers at launch = 64512; 256 x 208 + 128 x 80 = 63488 after the split.
 constexpr int kPaSoftmaxRegs = 208;
 constexpr int kPaOtherRegs = 80;
+// What the largest weight of a row is at least, as a power of two (see Sums).
+template <bool BF16> constexpr float kPaLift = BF16 ? 0.f : 7.f;
 constexpr uint32_t kPaColO = 256;                        // TMEM columns: S0 0, S1 128, O0 256, O1 384
 // The cost axis counts thirds of a key of a step with two row tiles.  A step with one row
 // tile takes two thirds of that; what an item takes besides its steps (first scores, epilogue) is
@@ -424,7 +431,7 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
         const uint64_t sl2 = pack_f32x2(sl, sl);
         uint64_t ref2, sums;                                               // two fp32 sums
         // a row that has seen no key yet has m = -inf: 0 as the reference keeps exp2(-inf) = 0
-        auto set_ref = [&]() { const float ref = m == -INFINITY ? 0.f : -m * sl; ref2 = pack_f32x2(ref, ref); };
+        auto set_ref = [&]() { const float ref = m == -INFINITY ? 0.f : kPaLift<BF16> - m * sl; ref2 = pack_f32x2(ref, ref); };
         auto hand_over = [&](int half) {                                   // its product can start
           tmem_wait_st();
           tc_fence_before();
@@ -522,7 +529,7 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
       if (two || w == 0) {
         const bool whole = wk.slot < 0;
         const int64_t orow = (int64_t)(wk.q0 + tok) * p.n_q_heads + wk.h * p.group + (row - tok_in * p.group);
-        const float m2 = m == -INFINITY ? -INFINITY : m * sl;           // base-2 units
+        const float m2 = m == -INFINITY ? -INFINITY : m * sl - kPaLift<BF16>;   // base-2 units, what l counts in
         float wa = l > 0.f ? 1.f / l : 0.f, wb = 0.f;
         if (l != l) wa = l;                                            // NaN scores stay NaN
         if (p.more_late) asm volatile("griddepcontrol.wait;" ::: "memory");
