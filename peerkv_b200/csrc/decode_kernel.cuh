@@ -1135,6 +1135,9 @@ decode_partial_kernel(const __grid_constant__ CUtensorMap tm_k,
           mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
           mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
         }
+        // An fp16 P ends at 2^-24: its reference stands 2^15 below the largest weight, so that the many small
+        // weights behind a dominant key keep their bits (down to 2^-29 of it).  m, l and o all count from it.
+        if constexpr (KVT == kKvF16) { mx0 -= 15.f; mx1 -= 15.f; }
         const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
         const float al0 = fast_exp2(m0 - mn0), al1 = fast_exp2(m1 - mn1);
         m0 = mn0; m1 = mn1;

@@ -153,6 +153,8 @@ __global__ void __launch_bounds__(kPfThreads) prefill_partial_kernel(const Prefi
     }
     mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1)); mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
     mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1)); mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+    // an fp16 P ends at 2^-24: its reference stands 2^15 below the largest weight (m, l and o count from it)
+    if constexpr (!BF16) { mx0 -= 15.f; mx1 -= 15.f; }
     const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
     // a row that has seen no key yet keeps m = -inf: use 0 as the reference so exp2 stays finite
     const float ref0 = mn0 == -INFINITY ? 0.f : mn0, ref1 = mn1 == -INFINITY ? 0.f : mn1;
