@@ -390,7 +390,7 @@ int pkv_home_merge(pkv_exchange* x, int32_t batch, uint32_t wait_mask, void* out
  *   [hidden]; hidden a multiple of 8.  Replaces add_kernel + rmsnorm_kernel
  *   (csrc/peer_fused_decoder.cu:51-71, 87-95).
  * pkv_rope_append: qkv [batch, (n_q_heads + 2 n_kv_heads) * head_dim] (q heads, k heads,
- *   v heads); rotate-half RoPE at angle positions[b] * inv_freq[i] on q and k; q goes to
+ *   v heads); rotate-half RoPE at angle positions[b] * inv_freq[i] (reduced in 64 bits) on q and k; q goes to
  *   q_out [batch, n_q_heads, head_dim]; the rotated k and v are stored into the pools at
  *   page pages[b], token slot slots[b] (element strides as in pkv_kv_view); pools NULL =
  *   no append.  No counterpart in the reference (its layer has neither RoPE nor an

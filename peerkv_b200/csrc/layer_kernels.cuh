@@ -100,9 +100,11 @@ struct RopeParams {
 };
 
 // grid (B, Hq + 2 Hkv), D/2 threads.  Rotate-half RoPE (x1, x2 = the two halves of a head:
-// out1 = x1 cos - x2 sin, out2 = x2 cos + x1 sin, angle = position * inv_freq[i], fp32) on
-// the q and k heads; q goes to q_out, the rotated k and the plain v go straight into the
-// page slot of the pool.
+// out1 = x1 cos - x2 sin, out2 = x2 cos + x1 sin, angle = position * inv_freq[i]) on the q and k
+// heads; q goes to q_out, the rotated k and the plain v go straight into the page slot of the
+// pool.  The angle is reduced in fp64, as norm_rope_append_kernel does: what prompts leave in the
+// cache and what decode steps ask it with have to turn alike (an fp32 product of a position near
+// 2^20 is off by up to 0.03 rad).
 template <bool BF16>
 __global__ void rope_append_kernel(const RopeParams p) {
   using E = Elem16<BF16>;
@@ -124,9 +126,9 @@ __global__ void rope_append_kernel(const RopeParams p) {
       return;
     }
   }
-  const float ang = (float)p.positions[b] * p.inv_freq[i];
+  const double turns = (double)p.positions[b] * (double)p.inv_freq[i] * 0.15915494309189533577;   // / 2 pi
   float sn, cs;
-  sincosf(ang, &sn, &cs);
+  sincospif(2.f * (float)(turns - rint(turns)), &sn, &cs);
   float x1, x2;
   if constexpr (BF16) { x1 = __bfloat162float(src[i]); x2 = __bfloat162float(src[i + half]); }
   else { x1 = __half2float(src[i]); x2 = __half2float(src[i + half]); }

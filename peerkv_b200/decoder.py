@@ -103,9 +103,10 @@ def rope_inv_freq(head_dim: int, theta: float, device) -> torch.Tensor:
 
 
 def rope_tables(pos: torch.Tensor, head_dim: int, theta: float):
-    """cos / sin [B, 1, D/2] (fp32) for integer positions pos [B] (torch reference of the kernel)."""
-    ang = pos.to(torch.float32)[:, None] * rope_inv_freq(head_dim, theta, pos.device)[None, :]
-    return ang.cos()[:, None, :], ang.sin()[:, None, :]
+    """cos / sin [B, 1, D/2] (fp32) for integer positions pos [B] (torch reference of the kernel): the
+    frequencies are fp32, the angles fp64."""
+    ang = pos.double()[:, None] * rope_inv_freq(head_dim, theta, pos.device).double()[None, :]
+    return ang.cos().float()[:, None, :], ang.sin().float()[:, None, :]
 
 
 def rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
