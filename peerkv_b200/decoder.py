@@ -184,6 +184,7 @@ class DecodeStep:
             raise PeerKVError("a shared prefix lives on one GPU: it cannot be combined with a group")
         self.scale = 1.0 / math.sqrt(g.head_dim)
         self._graph = None
+        self._status = torch.zeros(1, dtype=torch.int32, device=self.dev)    # of the appends and the prefixes
         dev, dt = self.dev, torch.bfloat16 if weights is None else weights.embed.dtype
         self.q = torch.zeros(batch, g.n_q_heads, g.head_dim, dtype=dt, device=dev)
         self.args = [make_args(self.q, l, self.scale) for l in kv]
@@ -201,13 +202,21 @@ class DecodeStep:
             self.next = z(batch, d=torch.int64)
             self.inv_freq = rope_inv_freq(g.rotary_dim or g.head_dim, g.rope_theta, dev)
 
+    def status(self) -> int:
+        """Reads and clears the device status bits of this rank's launches since the last call (attention,
+        prefixes and appends; synchronises the current stream)."""
+        return (self.shard if self.group is None else self.group).status() | ops.read_status(self._status)
+
+    def raise_on_status(self):
+        ops.raise_on_bits(self.status())
+
     # -- attention of one layer ---------------------------------------------------------- #
     def _attend(self, li: int):
         L, st = _lib.lib(), ops._stream(self.dev)
         if self.prefix is not None:
             l, (pt, pl, go) = self.kv[li], self.prefix
             ops.decode_shared_prefix(self.q, l.pool[0], l.pool[1], pt, pl, l.table, l.lens, group_offsets=go,
-                                     scale=self.scale, out=self.ao, shard=self.shard)
+                                     scale=self.scale, out=self.ao, shard=self.shard, status=self._status)
         elif self.group is None:
             check(L.pkv_decode(self.shard._h, C.byref(self.args[li]), self.ao.data_ptr(), ops._DT[self.ao.dtype],
                                None, st))
@@ -234,7 +243,7 @@ class DecodeStep:
                 k, v, slot = (None, None, None) if pool is None else (pool[0], pool[1], pages * pool.shape[2] + slots)
                 ops.norm_rope_append(self.qkv, self.pos, self.inv_freq, g.n_q_heads, g.n_kv_heads, self.q, k, v, slot,
                                      q_weight=lw.q_norm, k_weight=lw.k_norm, eps=g.rms_eps,
-                                     interleaved=g.rope_interleaved)
+                                     interleaved=g.rope_interleaved, status=self._status)
             self._attend(li)
             torch.matmul(self.ao.view(self.B, -1), lw.wo, out=self.proj)
             add_rmsnorm(self.x, self.proj, lw.norm2, self.h, g.rms_eps)
@@ -298,12 +307,22 @@ class DecodeStep:
 class PromptStep:
     """Prompts through the model on one GPU: packed sequences of different lengths, whole or as the
     next chunk behind what the cache holds already.  Fills every layer's pages and returns the
-    logits of each sequence's last token."""
+    logits of each sequence's last token.  A slot or a page id outside the pools does not end a
+    step: it sets a bit of the step's status (see status(), raise_on_status())."""
 
     def __init__(self, g: LlamaGeometry, weights: ModelWeights, kv: List[ShardedKVLayer], device):
         self.g, self.w, self.kv = g, weights, kv
         self.dev = torch.device(device)
         self.inv_freq = rope_inv_freq(g.rotary_dim or g.head_dim, g.rope_theta, self.dev)
+        self._status = torch.zeros(1, dtype=torch.int32, device=self.dev)
+
+    def status(self) -> int:
+        """Reads and clears the device status bits of the steps since the last call (synchronises the
+        current stream)."""
+        return ops.read_status(self._status)
+
+    def raise_on_status(self):
+        ops.raise_on_bits(self.status())
 
     def step(self, tokens: torch.Tensor, positions: torch.Tensor, slot_mapping: torch.Tensor,
              cu_seqlens: torch.Tensor, seq_lens: torch.Tensor) -> torch.Tensor:
@@ -325,8 +344,8 @@ class PromptStep:
             q = qkv[:, :g.n_q_heads * g.head_dim].view(T, g.n_q_heads, g.head_dim)     # turned where it lies
             ops.norm_rope_append(qkv, positions, self.inv_freq, g.n_q_heads, g.n_kv_heads, q, l.pool[0], l.pool[1],
                                  slot_mapping, q_weight=lw.q_norm, k_weight=lw.k_norm, eps=g.rms_eps,
-                                 interleaved=g.rope_interleaved)
-            ao = ops.prefill_paged(q, l.pool[0], l.pool[1], l.table, seq_lens, cu_seqlens)
+                                 interleaved=g.rope_interleaved, status=self._status)
+            ao = ops.prefill_paged(q, l.pool[0], l.pool[1], l.table, seq_lens, cu_seqlens, status=self._status)
             add_rmsnorm(x, torch.matmul(ao.view(T, -1), lw.wo), lw.norm2, h, g.rms_eps)
             swiglu(torch.matmul(h, lw.w_gate_up), act)
             delta = torch.matmul(act, lw.w_down)

@@ -30,6 +30,22 @@ def _require_cuda(t: torch.Tensor, name: str):
         raise PeerKVError(f"{name} must be a CUDA tensor (this package has no CPU path)")
 
 
+def raise_on_bits(status: int):
+    """PeerKVError that says what the bits of a device status word mean, if any is set."""
+    if status:
+        names = [n for b, n in ((1, "pipeline wait timed out"), (2, "block-table id outside the pool"),
+                                (4, "query never arrived"), (8, "a peer partial never arrived")) if status & b]
+        raise PeerKVError("device status 0x%x: %s" % (status, "; ".join(names)))
+
+
+def read_status(word: torch.Tensor) -> int:
+    """Reads and clears a status tensor (int32 [1]) that calls were given; synchronises the current stream."""
+    bits = int(word[0])
+    if bits:
+        word.zero_()
+    return bits
+
+
 class Shard:
     """One GPU's attention context: persistent split-K scratch and status word
     (replaces the per-call scratch of PeerKV csrc/peer_fused_attn_ext.cu:56-63)."""
@@ -75,11 +91,7 @@ class Shard:
         return {"launches": int(a.value), "kv_bytes_read": kv_bytes}
 
     def raise_on_status(self):
-        st = self.status()
-        if st:
-            names = [n for b, n in ((1, "pipeline wait timed out"), (2, "block-table id outside the pool"),
-                                    (4, "query never arrived"), (8, "a peer partial never arrived")) if st & b]
-            raise PeerKVError("device status 0x%x: %s" % (st, "; ".join(names)))
+        raise_on_bits(self.status())
 
 
 _shards = {}
@@ -420,7 +432,8 @@ def prefill_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, b
     [total_q, Hq] fp32, so that shards merge with merge_partials.  Rows that see nothing are 0 with
     lse -inf; rows behind the last sequence are not written.  V of every token of a sequence
     must be finite; what the pages hold behind a sequence does not matter.
-    `status` (int32 [1] on q's GPU) gets the device status bits OR-ed in."""
+    `status` (int32 [1] on q's GPU) gets the device status bits OR-ed in (read_status, raise_on_bits);
+    without one a page id outside the pool, read as page 0, goes unreported."""
     q = _check_prompt_q(q)
     cu = _cu(cu_seqlens_q, q.device, "cu_seqlens_q")
     n = cu.numel() - 1
