@@ -339,7 +339,8 @@ def _prompt_workspace(device: torch.device, more: int = 0) -> torch.Tensor:
 
 def _rows_of_heads(t: torch.Tensor, name: str) -> torch.Tensor:
     """[tokens, heads, 128] as the kernels read it: unit last stride, the others positive
-    multiples of 8 elements, 16-byte aligned; anything else is copied."""
+    multiples of 8 elements, 16-byte aligned; anything else is copied (contiguous() would return a
+    contiguous tensor with a misaligned start as it is)."""
     shape = t.shape
     if len(shape) != 3 or shape[2] != HEAD_DIM:
         raise PeerKVError(f"{name} must be [tokens, heads, {HEAD_DIM}]; got {tuple(shape)}")
@@ -347,7 +348,7 @@ def _rows_of_heads(t: torch.Tensor, name: str) -> torch.Tensor:
     s0, s1, s2 = t.stride()
     ok = s2 == 1 and t.data_ptr() % 16 == 0 and (n0 <= 1 or (s0 > 0 and s0 % 8 == 0)) and \
         (n1 <= 1 or (s1 > 0 and s1 % 8 == 0))
-    return t if ok or t.numel() == 0 else t.contiguous()
+    return t if ok or t.numel() == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _status_word(status: Optional[torch.Tensor], device: torch.device):
@@ -596,7 +597,7 @@ def norm_rope_append(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: Optio
     T = shape[0]
     qkv_ptr = qkv.data_ptr()
     if T and (st[1] != 1 or st[0] % 8 or qkv_ptr % 16):
-        qkv = qkv.contiguous()
+        qkv = qkv.clone(memory_format=torch.contiguous_format)        # (contiguous() keeps a misaligned start)
         qkv_ptr, st = qkv.data_ptr(), qkv.stride()
     if q_out is None:
         q_out = qkv.new_empty((T, n_q_heads, HEAD_DIM))
