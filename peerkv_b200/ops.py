@@ -374,8 +374,10 @@ def _prompt_call(q, view, scale, causal, out, lse, cu_q, n_seqs, status, block_t
     total_q, n_heads, _ = q.shape
     st = q.stride()
     paged = block_table is not None
+    # (a table without columns has no memory; its rows have room for no token, and nothing is read)
+    table = None if not paged else block_table.data_ptr() or cu_q.data_ptr()
     a = _lib.PromptArgs(q.data_ptr(), st[0], st[1], _DT[q.dtype], n_heads, total_q, n_seqs, cu_q.data_ptr(), view,
-                        block_table.data_ptr() if paged else None, block_table.stride(0) if paged else 0,
+                        table, block_table.stride(0) if paged else 0,
                         block_table.shape[1] if paged else 0, 1 if causal else 0,
                         seq_lens.data_ptr() if paged else None, None if paged else cu_k.data_ptr(),
                         more[0], more[1], scale, 0 if more[0] is None else 1)
@@ -415,7 +417,7 @@ def _table(block_table, device, rows: int, name: str) -> torch.Tensor:
     shape = bt.shape
     if len(shape) != 2 or shape[0] != rows:
         raise PeerKVError(f"{name} must be [{rows}, pages]; got {tuple(shape)}")
-    return bt if shape[1] > 0 else bt.new_zeros(rows, 1)
+    return bt
 
 
 def prefill_paged(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
@@ -514,6 +516,8 @@ def decode_shared_prefix(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     bt, sl = _table(block_table, dev, B, "block_table"), _meta(seq_lens, dev, "seq_lens")
     if sl.dim() != 1 or sl.numel() != B:
         raise PeerKVError(f"seq_lens must be [{B}]; got {tuple(sl.shape)}")
+    if bt.shape[1] == 0:                               # no room for own tokens, whatever seq_lens says
+        bt, sl = bt.new_zeros(B, 1), torch.zeros_like(sl)
     view = _prompt_pool(q, k_pool, v_pool)
     out = _check_out(out, q)
     lse = q.new_empty((B, Hq), dtype=torch.float32) if return_lse else None
