@@ -491,11 +491,12 @@ def decode_shared_prefix(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     prefix is read once for its group instead of once per sequence.
 
     q [batch, Hq, 128]; group g owns sequences group_offsets[g] .. group_offsets[g+1] - 1 (default:
-    one group of all; the offsets run from 0 to batch) and the prefix of prefix_lens[g]
-    tokens in the pages prefix_table[g] (any length, 0 allowed).  block_table / seq_lens
+    one group of all; the offsets run from 0 to batch, rows of no group are not written) and the prefix of
+    prefix_lens[g] tokens in the pages prefix_table[g] (any length, 0 allowed).  block_table / seq_lens
     describe what each sequence has of its own behind the prefix (0 tokens allowed), e.g.
     the columns of a full table behind the shared pages.  Result as decode_paged over prefix
-    and own tokens: out [batch, Hq, 128], with return_lse the lse [batch, Hq].
+    and own tokens: out [batch, Hq, 128], with return_lse the lse [batch, Hq].  As decode_paged it takes
+    at most 8 query heads per kv-head; pages hold a multiple of 16 tokens of q's type.
     The own tokens go through `shard` (see decode_paged), whose launches must not overlap and which
     reports their bad pages; `status` gets those of the prefixes."""
     q = _check_prompt_q(q)
@@ -509,6 +510,8 @@ def decode_shared_prefix(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
         go = torch.arange(0, B + 1, B, dtype=torch.int32, device=dev) if B else \
             torch.zeros(2, dtype=torch.int32, device=dev)
     n = go.numel() - 1
+    if n == 0 and B > 0:
+        raise PeerKVError(f"group_offsets describe no group, and q has {B} rows")
     pt = _table(pt, dev, n, "prefix_table")
     pl = _meta(prefix_lens, dev, "prefix_lens").reshape(-1)
     if pl.numel() != n:
