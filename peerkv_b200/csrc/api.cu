@@ -1481,6 +1481,8 @@ extern "C" int pkv_norm_rope_append(int device, const pkv_append_args* a, uint32
   if (a->n_tokens == 0) return PKV_OK;
   if (!a->qkv || !a->q_out || (a->rot_dim > 0 && (!a->positions || !a->inv_freq))) return fail(PKV_E_INVALID, "null pointer");
   if (a->qkv_stride % 8 || a->q_out_stride % 8) return fail(PKV_E_INVALID, "token strides must be multiples of 8 elements");
+  if (a->n_tokens > 1 && a->q_out_stride < (int64_t)a->n_q_heads * pkv::kHeadDim)
+    return fail(PKV_E_INVALID, "q_out_stride %lld: tokens of q_out must not overlap", (long long)a->q_out_stride);
   if ((reinterpret_cast<uintptr_t>(a->qkv) | reinterpret_cast<uintptr_t>(a->q_out) | reinterpret_cast<uintptr_t>(a->q_weight) |
        reinterpret_cast<uintptr_t>(a->k_weight)) & 15)
     return fail(PKV_E_INVALID, "qkv, q_out and the weights must be 16-byte aligned");
