@@ -86,8 +86,8 @@ typedef struct pkv_kv_view {
  *                (0 allowed; only a sequence's last listed page may be partial)
  *   scale        softmax scale (the reference default is 1/sqrt(head_dim))
  *   early_dependent  1: the kernel behind this one may take SMs as they become free (see more_late
- *                in pkv_prompt_args; of no use for anything else), and the work is split evenly
- *                instead of by how long the shard's last launch took */
+ *                in pkv_prompt_args; of no use for anything else), and the work is split by
+ *                the lengths alone instead of by how long the shard's last launch took */
 typedef struct pkv_decode_args {
   const void* q;
   int32_t q_dtype;

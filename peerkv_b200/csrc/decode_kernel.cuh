@@ -74,7 +74,7 @@ struct DecodeParams {
   int head_major;      // 1: pool dims are (d, tok, head, page); 0: (d, head, tok, page)
   int n_cta_x;
   int force_empty;     // 1: the pool holds no page; every sequence counts as empty here
-  int early_dependent; // 1: the kernel behind this one may take its SMs as they become free
+  int early_dependent; // 1: the kernel behind this one may take its SMs as they become free; fixed split
   float scale_log2;    // softmax scale * log2(e)
   float* part_o;       // [slots][Hq][128]
   float* part_ml;      // [slots][Hq][2]  (m in log2 units, l)
@@ -529,6 +529,32 @@ __device__ __forceinline__ void build_cta_bounds(int* bound, float* wtmp, int to
   bar_sync(1, nthr);
 }
 
+// The same for a launch that learns from none before it: the bounds follow from the lengths alone.  What a sequence
+// costs a CTA besides its tiles (its query, the flush, the merge) counts like kSeqCost tiles.  128 short
+// sequences behind three prefixes, 8.5 tiles a CTA: 112 us in a graph, 113 / 122 / 121 with 4 / 2 / 1 and 111
+// with 10, 136 when only tiles count (122 when learned from the launch before); 64 sequences, 15.5 tiles a CTA:
+// 94 us, 100 with 4, 94 with 10, 100 when only tiles count.  With less than a tile per CTA they are dealt
+// out one each (25.8 us for 4 sequences; 26.5 by cost).
+constexpr int kSeqCost = 6;
+__device__ __forceinline__ void build_fixed_bounds(int* bound, const int* prefix, int batch, int n_cta, int nthr) {
+  const int total = prefix[batch];
+  const int64_t cost = total + (int64_t)kSeqCost * batch;
+  for (int c = threadIdx.x; c <= n_cta; c += nthr) {
+    if (total <= n_cta || c == n_cta) {
+      bound[c] = c == n_cta ? total : min(c, total);
+      continue;
+    }
+    const int x = (int)(cost * c / n_cta);
+    int lo = 0, hi = batch;                      // largest s that starts at or before x on the axis of costs
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (prefix[mid] + kSeqCost * mid <= x) lo = mid; else hi = mid;
+    }
+    bound[c] = min(prefix[lo + 1], max(prefix[lo], x - kSeqCost * (lo + 1)));
+  }
+  bar_sync(1, nthr);
+}
+
 // The CTA whose range holds tile g: largest c with bound[c] <= g.
 __device__ __forceinline__ int find_cta(const int* bound, int n_cta, int g) {
   int lo = 0, hi = n_cta;
@@ -700,7 +726,8 @@ decode_partial_kernel(const __grid_constant__ CUtensorMap tm_k,
   } else {
     build_tile_prefix(prefix, p.seq_lens, p.batch, p.page_size, p.tiles_per_page, p.force_empty != 0,
                       kWorkThreads);
-    build_cta_bounds(bound, cta_weight, prefix[p.batch], p.n_cta_x, p.obs_read, kWorkThreads);
+    if (p.early_dependent) build_fixed_bounds(bound, prefix, p.batch, p.n_cta_x, kWorkThreads);
+    else build_cta_bounds(bound, cta_weight, prefix[p.batch], p.n_cta_x, p.obs_read, kWorkThreads);
     __threadfence_block();
     bar_arrive(2, kWorkThreads + 32);
   }
