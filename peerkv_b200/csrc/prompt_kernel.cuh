@@ -39,9 +39,10 @@
 // What bounds it (B200, bf16, 32 q and 8 kv heads).  A step, 256 rows x 128 keys, takes the tensor
 // cores 2048 cycles and the special-function unit as many (32768 exponentials at 16 a cycle); it
 // measures 2900: a stream's scores, exponentials and product follow one another, and two streams
-// half a step apart hide most but not all of that.  8192-token prompt: 455 us (1.2 PFLOP/s, 0.75
-// of the measured burst rate of the library's large products, 0.88 of the sustained one; the
-// clock is down to 1.5 GHz under the power cap).  Short prompts and short prefixes are bound by
+// half a step apart hide most but not all of that (the tensor pipe is busy 54 % of the active cycles, the
+// special-function unit 57 %).  8192-token prompt: 532 us call behind call (1.03 PFLOP/s, 0.75 of the
+// sustained rate of the library's large products; the power cap takes the clock down), 475 us from
+// idle (1.16 PFLOP/s, 0.72 of their burst rate).  Short prompts and short prefixes are bound by
 // latency: 6 us from launch to the first scores (lengths, block table, first tiles, each a trip to
 // memory behind the other), 2 us an item's epilogue, 5 us the join.  A prefix of 32768 tokens for 64
 // sequences streams at 3 TB/s: its steps are compute, then the same latencies.
@@ -74,9 +75,10 @@ template <bool BF16> constexpr float kPaLift = BF16 ? 0.f : 7.f;
 constexpr uint32_t kPaColO = 256;                        // TMEM columns: S0 0, S1 128, O0 256, O1 384
 // The cost axis counts thirds of a key of a step with two row tiles.  A step with one row
 // tile takes two thirds of that; what an item takes besides its steps (first scores, epilogue) is
-// weighted like three steps (192 keys instead of 384 left ragged batches 10 % out of balance).
+// weighted like three steps (with 192 keys instead of 384 a ragged batch of prompts takes 370 us instead of 349, a chunk
+// that rides with single tokens 73 instead of 66).
 constexpr int kPaItemCost = 1152;  // per item, = 3 x 384 keys
-constexpr int kPaMinPiece = 1024;  // no CTA gets less (2048-token prefix: 34 us; 35 with 768, 36 with 1536)
+constexpr int kPaMinPiece = 1024;  // no CTA gets less (4 sequences behind 2048 tokens: 24.9 us in a graph; 25.6 with 768, 26.1 with 1536)
 
 // Which CTA found which item cut (one per CTA, for the join).
 struct PromptRec {
@@ -940,7 +942,7 @@ prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_consta
 // 4 KB runs.  The pieces are a few MB that were written a moment ago: L2.
 constexpr int kPjTasks = 16;
 // Pieces in flight per thread: a join is a few trips to the L2, not one per piece.  (4: packed short prompts
-// 28.2 us instead of 29.2, but 64 sequences behind 32768 tokens, 18 pieces an item, 103.6 instead of 101.7.)
+// 28.8 us instead of 29.6, but 64 sequences behind 32768 tokens, 18 pieces an item, 2.4 us more.)
 constexpr int kPjBatch = 8;
 __global__ void __launch_bounds__(256) prompt_join_kernel(const PromptParams p, int n_grid) {
   __shared__ int64_t s_a[kPaMaxCtas];
