@@ -60,6 +60,7 @@ class Shard:
         h = C.c_void_p()
         check(_lib.lib().pkv_shard_create(C.byref(h), self.device.index, self.max_batch, self.n_q_heads))
         self._h = h
+        self.captured = False          # a CUDA graph may hold launches on this context (see get_shard)
 
     def close(self):
         if getattr(self, "_h", None):
@@ -96,12 +97,14 @@ class Shard:
 
 _shards = {}
 _retired = []          # (shard, event): outgrown contexts whose scratch queued kernels may still use
+_kept = []             # outgrown contexts that graphs were captured with: those may be replayed at any time
 
 
 def get_shard(device: torch.device, batch: int, n_q_heads: int) -> Shard:
     """Cached per (device, n_q_heads); regrown when a larger batch shows up.  The outgrown
     context is not freed under kernels that may still be queued on it, and the host does
-    not wait for them either: it is retired with an event and freed once that has passed."""
+    not wait for them either: it is retired with an event and freed once that has passed.  One
+    that was handed out during a capture lives as long as the process."""
     device = torch.device(device)
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
@@ -112,7 +115,9 @@ def get_shard(device: torch.device, batch: int, n_q_heads: int) -> Shard:
             _retired.remove(item)
     s = _shards.get(key)
     if s is None or s.max_batch < batch:
-        if s is not None:
+        if s is not None and s.captured:
+            _kept.append(s)
+        elif s is not None:
             ev = torch.cuda.Event()
             with torch.cuda.device(device):
                 ev.record(torch.cuda.current_stream(device))
@@ -120,6 +125,8 @@ def get_shard(device: torch.device, batch: int, n_q_heads: int) -> Shard:
         cap = min(4096, max(64, 1 << max(0, batch - 1).bit_length()))   # next power of two, 64..4096
         s = Shard(device, max(cap, batch), n_q_heads)                    # > 4096: let the library refuse it
         _shards[key] = s
+    if not s.captured and torch.cuda.is_current_stream_capturing():
+        s.captured = True
     return s
 
 
