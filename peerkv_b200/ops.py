@@ -500,8 +500,8 @@ def decode_shared_prefix(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     q [batch, Hq, 128]; group g owns sequences group_offsets[g] .. group_offsets[g+1] - 1 (default:
     one group of all; the offsets run from 0 to batch, rows of no group are not written) and the prefix of
     prefix_lens[g] tokens in the pages prefix_table[g] (any length, 0 allowed).  block_table / seq_lens
-    describe what each sequence has of its own behind the prefix (0 tokens allowed), e.g.
-    the columns of a full table behind the shared pages.  Result as decode_paged over prefix
+    describe what each sequence has of its own behind the prefix (0 tokens allowed; as in decode_paged
+    every page of a length must stand in its row), e.g. the columns of a full table behind the shared pages.  Result as decode_paged over prefix
     and own tokens: out [batch, Hq, 128], with return_lse the lse [batch, Hq].  As decode_paged it takes
     at most 8 query heads per kv-head; pages hold a multiple of 16 tokens of q's type.
     The own tokens go through `shard` (see decode_paged), whose launches must not overlap and which
